@@ -1,0 +1,521 @@
+"""Timed cases of the policy operators: what a program that trains a model's
+decisions (boosted trees with caller gradients, or any model with margins over
+classes) calls between two steps of the model.
+
+Kinds of case (``kind``):
+
+logprobs     log-probability of the action taken in every row of margins, with
+             the distribution's entropy if asked for; with ``backward`` also the
+             gradient of the margins from the gradients of both.
+policy       clipped policy loss with a KL term to a reference and an entropy
+             bonus: the rows' losses and the gradient (and hessian) of the
+             margins.
+preference   preference loss of pairs of sequences (paired log ratios): the
+             pairs' losses and the gradient (and hessian) of the margins.
+recurrence   gated linear recurrence over time (advantages are its reverse
+             direction with one channel); with ``backward`` its gradients.
+
+A row whose action is -1, or whose weight is 0, is not counted: its margins may
+hold anything (here: NaN) and its gradient is zero.
+"""
+import functools
+import math
+import os
+import sys
+
+import torch
+
+own = False
+DEVICE = "cuda:0"
+
+
+# ---------------------------------------------------------------------------
+# Cases
+# ---------------------------------------------------------------------------
+def listed():
+    return [
+        # One decision of a ten-class model, served with its log-probability: latency.
+        logprobs("score_one", 1, 10, "float32", entropy=True),
+        # Scoring a batch of tokens with the reference model, an odd vocabulary.
+        logprobs("score_4k_wide", 4096, 50021, "bfloat16"),
+        # A custom loss on the margins of the ten-class table: forward and backward.
+        logprobs("logprobs_grad_60k", 60_000, 10, "float32", entropy=True, backward=True),
+        # One boosting round's gradients of a small table with four actions.
+        policy("policy_10k", 10_000, 4, "float32", hessian=True, illegal=0.1),
+        # The same for a million decisions among ten classes.
+        policy("policy_1m", 1_000_000, 10, "float32", hessian=True),
+        # A training batch of tokens over a whole vocabulary.
+        policy("policy_8k_wide", 8192, 32768, "bfloat16"),
+        # A few tokens over a very wide odd vocabulary: less rows than compute units.
+        policy("policy_24_long", 24, 131071, "float32", illegal=0.3),
+        # Preferences between episodes of tree decisions, with hessians for the booster.
+        preference("preference_60k", 60_000, 500, 10, "float32", hessian=True),
+        # Preferences between sequences of tokens.
+        preference("preference_16k_wide", 16_384, 16, 32_000, "bfloat16"),
+        # Advantages of a small batch of episodes: reverse scan of one channel.
+        recurrence("advantages_64", 64, 1000, 1, "float32", reverse=True),
+        # A recurrent layer's forward pass over a batch of sequences.
+        recurrence("recurrence_8x4k", 8, 4096, 2048, "bfloat16"),
+        # A recurrent layer's backward pass over long sequences.
+        recurrence("recurrence_grad_32k", 4, 32_768, 512, "float32", backward=True),
+    ]
+
+
+def draw(rng):
+    def log(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    kind = rng.choice(["logprobs", "policy", "policy", "preference", "recurrence", "recurrence"])
+    dtype = rng.choice(["float32", "bfloat16", "float16"])
+    if kind == "recurrence":
+        t = log(1, 200_000)
+        c = rng.choice([1, log(2, 4096)])
+        b = max(1, min(log(1, 4096), 60_000_000 // (t * c)))
+        t = min(t, 60_000_000 // c)
+        return recurrence(None, b, t, c, dtype, reverse=rng.random() < 0.5,
+                          backward=rng.random() < 0.5)
+    k = rng.choice([log(2, 64), log(64, 4096), log(4096, 140_000)])
+    n = max(1, min(log(1, 1_000_000), 250_000_000 // k))
+    hessian = dtype == "float32" and rng.random() < 0.5
+    if kind == "logprobs":
+        return logprobs(None, n, k, dtype, entropy=rng.random() < 0.5,
+                        backward=rng.random() < 0.5)
+    if kind == "policy":
+        return policy(None, n, k, dtype, hessian=hessian, illegal=rng.choice([0.0, 0.3]),
+                      clip_high=rng.choice([0.2, 0.28]), kl=rng.choice([0.0, 0.05]),
+                      entropy=rng.choice([0.0, 0.01]))
+    return preference(None, n, max(1, n // log(2, 2000)), k, dtype, hessian=hessian,
+                      average=rng.random() < 0.3, smoothing=rng.choice([0.0, 0.1]))
+
+
+def logprobs(name, rows, classes, dtype, entropy=False, backward=False):
+    return _named(name, {"kind": "logprobs", "rows": rows, "classes": classes, "dtype": dtype,
+                         "entropy": entropy, "backward": backward})
+
+
+def policy(name, rows, classes, dtype, hessian=False, illegal=0.0, clip_low=0.2, clip_high=0.2,
+           kl=0.05, entropy=0.01):
+    return _named(name, {"kind": "policy", "rows": rows, "classes": classes, "dtype": dtype,
+                         "hessian": hessian, "illegal": illegal, "clip_low": clip_low,
+                         "clip_high": clip_high, "kl": kl, "entropy": entropy})
+
+
+def preference(name, rows, pairs, classes, dtype, hessian=False, average=False, smoothing=0.0,
+               beta=0.1):
+    return _named(name, {"kind": "preference", "rows": rows, "pairs": pairs, "classes": classes,
+                         "dtype": dtype, "hessian": hessian, "average": average,
+                         "smoothing": smoothing, "beta": beta})
+
+
+def recurrence(name, batch, time, channels, dtype, reverse=False, backward=False):
+    return _named(name, {"kind": "recurrence", "batch": batch, "time": time,
+                         "channels": channels, "dtype": dtype, "reverse": reverse,
+                         "backward": backward})
+
+
+def _named(name, case):
+    return case if name is None else {"name": name, **case}
+
+
+# ---------------------------------------------------------------------------
+# Inputs
+# ---------------------------------------------------------------------------
+def prepare(case, seed):
+    g = torch.Generator(device=DEVICE)
+    g.manual_seed(seed)
+    dtype = getattr(torch, case["dtype"])
+
+    def normal(*shape, scale=1.0):
+        return torch.randn(shape, generator=g, device=DEVICE) * scale
+
+    def uniform(*shape):
+        return torch.rand(shape, generator=g, device=DEVICE)
+
+    state = {"case": dict(case)}
+    if case["kind"] == "recurrence":
+        shape = (case["batch"], case["time"], case["channels"])
+        gate = torch.sigmoid(normal(*shape) + 3.0)
+        gate[uniform(*shape) < 0.002] = 0.0  # an episode ends, a feature is reset
+        value = normal(*shape) * (1.0 - gate)
+        state["gate"], state["initial"] = gate.to(dtype), normal(shape[0], shape[2])
+        if case["backward"]:
+            # The states that the forward pass left, and their gradients.
+            states, _ = _recur(state["gate"].float(), value, state["initial"], case["reverse"])
+            state["states"] = states.to(dtype)
+            state["dstates"] = normal(*shape).to(dtype)
+            state["dlast"] = normal(shape[0], shape[2])
+        else:
+            state["value"] = value.to(dtype)
+        return state
+    n, k = case["rows"], case["classes"]
+    margin = normal(n, k, scale=2.0)
+    action = torch.randint(k, (n,), generator=g, device=DEVICE)
+    if case.get("illegal"):
+        legal = torch.rand((n, k), generator=g, device=DEVICE) >= case["illegal"]
+        legal.scatter_(1, action[:, None], True)
+        margin.masked_fill_(~legal, -math.inf)
+    state["margin"] = margin = margin.to(dtype)
+    wide = margin.float()
+    logp = torch.gather(wide, 1, action[:, None])[:, 0] - torch.logsumexp(wide, 1)
+    del wide
+    skipped = uniform(n) < 0.05  # padding
+    skipped[0] = False
+    state["action"] = action
+    if case["kind"] == "policy":
+        state["weight"] = torch.where(skipped, 0.0, 1.0)
+        state["old_logp"] = logp + normal(n, scale=0.15)
+        state["reference"] = logp + normal(n, scale=0.2)
+        state["advantage"] = normal(n)
+    else:
+        action[skipped] = -1
+        if case["kind"] == "logprobs":
+            state["dlogp"], state["dentropy"] = normal(n), normal(n, scale=0.01)
+        else:
+            state["reference"] = logp + normal(n, scale=0.2)
+            count = 2 * case["pairs"]
+            cut = torch.arange(1, count, device=DEVICE) + (uniform(count - 1) - 0.5) * 0.9
+            cut = (cut.double() * (n / count)).round().long().clamp(0, n)
+            ends = torch.tensor([0, n], device=DEVICE)
+            state["sequences"] = torch.cat([ends[:1], cut, ends[1:]])
+    margin[skipped] = math.nan
+    return state
+
+
+# ---------------------------------------------------------------------------
+# One pass
+# ---------------------------------------------------------------------------
+def run(state):
+    case = state["case"]
+    return {"logprobs": _run_logprobs, "policy": _run_policy, "preference": _run_preference,
+            "recurrence": _run_recurrence}[case["kind"]](state, case)
+
+
+@functools.lru_cache(maxsize=None)
+def _kept():
+    """The operators and the workspace that a program keeps for its calls."""
+    path = os.path.join(os.getcwd(), "decision-programs_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from dpgbdt import ops
+
+    return ops, ops.Workspace()
+
+
+def _softmax(margin, counted):
+    """(margins, their maximum, the logarithm of the sum of exponentials (added up in 64 bits:
+    sequences add thousands of them), log-probabilities, probabilities)."""
+    z = torch.where(counted[:, None], margin.float(), 0.0)
+    top = z.amax(1, keepdim=True)
+    shifted = z - top
+    logs = torch.exp(shifted).sum(1, keepdim=True, dtype=torch.float64).log()
+    logps = shifted - logs.float()
+    return z, top, logs, logps, torch.exp(logps)
+
+
+def _taken(z, top, logs, action):
+    """Log-probability of the action of every row, in 64 bits."""
+    zy = torch.gather(z, 1, action[:, None])
+    return ((zy.double() - top.double()) - logs)[:, 0]
+
+
+def _entropy(logps, p):
+    return -torch.where(p > 0, p * logps, 0.0).sum(1)
+
+
+def _add_choice(grad, action, c):
+    return grad.scatter_add_(1, action[:, None], c[:, None])
+
+
+def _hessian(p, c, counted):
+    h = torch.clamp(2.0 * c[:, None] * p * (1.0 - p), min=1e-16)
+    return torch.where(counted[:, None], h, 0.0)
+
+
+def _run_logprobs(state, case):
+    margin, action = state["margin"], state["action"]
+    if own:
+        ops, ws = _kept()
+        logp, entropy = ops.action_logprobs(ws, margin, action, entropy=case["entropy"])
+        out = {"logp": logp, "entropy": entropy}
+        if case["backward"]:
+            out["grad"] = ops.action_logprobs_backward(
+                ws, margin, action, state["dlogp"], state["dentropy"] if case["entropy"] else None)
+        return out
+    counted = action >= 0
+    y = action.clamp(min=0)
+    z, top, logs, logps, p = _softmax(margin, counted)
+    logp = torch.where(counted, _taken(z, top, logs, y), 0.0).float()
+    entropy = torch.where(counted, _entropy(logps, p), 0.0) if case["entropy"] else None
+    out = {"logp": logp, "entropy": entropy}
+    if case["backward"]:
+        c = torch.where(counted, state["dlogp"], 0.0)
+        grad = -c[:, None] * p
+        if case["entropy"]:
+            d = torch.where(counted, state["dentropy"], 0.0)
+            grad = grad - d[:, None] * torch.where(p > 0, p * (logps + entropy[:, None]), 0.0)
+        out["grad"] = _add_choice(grad, y, c).to(margin.dtype)
+    return out
+
+
+def _run_policy(state, case):
+    margin, action, weight = state["margin"], state["action"], state["weight"]
+    old, ref, adv = state["old_logp"], state["reference"], state["advantage"]
+    if own:
+        ops, ws = _kept()
+        loss, logp, kl, entropy, grad, hess = ops.policy_loss(
+            ws, margin, action, old, adv, weight=weight, reference=ref,
+            clip_low=case["clip_low"], clip_high=case["clip_high"], kl=case["kl"],
+            entropy=case["entropy"], hessian=case["hessian"])
+        return {"loss": loss, "logp": logp, "kl": kl, "entropy": entropy, "grad": grad,
+                "hess": hess}
+    counted = weight != 0
+    z, top, logs, logps, p = _softmax(margin, counted)
+    logp = _taken(z, top, logs, action)
+    # The ratio is clipped where it passes the border on the advantage's side.  Rows that 32
+    # bits cannot decide are looked at in 64.
+    high, low = math.log1p(case["clip_high"]), math.log1p(-case["clip_low"])
+    border = torch.where(adv > 0, high, low)
+    gap = logp - old.double() - border
+    near = ((gap.abs() < 1e-5) & counted).nonzero()[:, 0]
+    some = z[near].double()
+    gap[near] = (torch.gather(some, 1, action[near, None])[:, 0] - some.amax(1)
+                 - torch.exp(some - some.amax(1, keepdim=True)).sum(1).log()
+                 - old[near].double() - border[near])
+    active = torch.where(adv > 0, gap < 0, gap > 0)
+    ratio = torch.exp(logp - old.double()).float()
+    clipped = ratio.clamp(1.0 - case["clip_low"], 1.0 + case["clip_high"])
+    d = ref.double() - logp
+    kl = torch.where(counted, torch.expm1(d) - d, 0.0).float()
+    entropy = torch.where(counted, _entropy(logps, p), 0.0)
+    loss = -torch.minimum(ratio * adv, clipped * adv) + case["kl"] * kl - case["entropy"] * entropy
+    c = -ratio * adv * active - case["kl"] * torch.expm1(d).float()
+    c = torch.where(counted, c * weight, 0.0)
+    bonus = torch.where(counted, case["entropy"] * weight, 0.0)
+    tilt = torch.where(p > 0, p * (logps + entropy[:, None]), 0.0)
+    grad = _add_choice(bonus[:, None] * tilt - c[:, None] * p, action, c)
+    return {"loss": torch.where(counted, loss * weight, 0.0),
+            "logp": torch.where(counted, logp, 0.0).float(), "kl": kl, "entropy": entropy,
+            "grad": grad.to(margin.dtype),
+            "hess": _hessian(p, c.abs() + bonus, counted) if case["hessian"] else None}
+
+
+def _run_preference(state, case):
+    margin, action, ref, ptr = (state["margin"], state["action"], state["reference"],
+                                state["sequences"])
+    if own:
+        ops, ws = _kept()
+        loss, score, logp, grad, hess = ops.preference_loss(
+            ws, margin, action, ptr, reference=ref, beta=case["beta"],
+            smoothing=case["smoothing"], average=case["average"], hessian=case["hessian"])
+        return {"loss": loss, "score": score, "logp": logp, "grad": grad, "hess": hess}
+    counted = action >= 0
+    y = action.clamp(min=0)
+    z, top, logs, logps, p = _softmax(margin, counted)
+    logp = torch.where(counted, _taken(z, top, logs, y), 0.0)
+    # Sums over the sequences, in 64 bits: differences of a running sum.
+    over = torch.zeros(len(logp) + 1, dtype=torch.float64, device=logp.device)
+    over[1:] = torch.where(counted, logp - ref.double(), 0.0).cumsum(0)
+    total = over[ptr[1:]] - over[ptr[:-1]]
+    share = torch.ones_like(total)
+    if case["average"]:
+        over[1:] = counted.double().cumsum(0)
+        share = 1.0 / (over[ptr[1:]] - over[ptr[:-1]]).clamp(min=1.0)
+    score = case["beta"] * (total[0::2] * share[0::2] - total[1::2] * share[1::2])
+    e = case["smoothing"]
+    loss = (1 - e) * _softplus(-score) + e * _softplus(score)
+    slope = case["beta"] * (e / (1 + torch.exp(-score)) - (1 - e) / (1 + torch.exp(score)))
+    slope = torch.stack([slope, -slope], 1).flatten() * share
+    of_row = torch.repeat_interleave(slope, ptr[1:] - ptr[:-1])
+    c = torch.where(counted, of_row, 0.0).float()
+    grad = _add_choice(-c[:, None] * p, y, c)
+    return {"loss": loss.float(), "score": score.float(), "logp": logp.float(),
+            "grad": grad.to(margin.dtype),
+            "hess": _hessian(p, c.abs(), counted) if case["hessian"] else None}
+
+
+def _softplus(x):
+    return x.clamp(min=0.0) + torch.log1p(torch.exp(-x.abs()))
+
+
+def _recur(gate, value, initial, reverse):
+    """States of the recurrence in 32 bits, and the last one: pairs (gate, value) of
+    neighbouring spans are joined, spans doubling (no division: gates may be zero)."""
+    if reverse:
+        gate, value = gate.flip(1), value.flip(1)
+    a, b, span = gate, value, 1
+    while span < a.shape[1]:
+        b = torch.cat([b[:, :span], b[:, span:] + a[:, span:] * b[:, :-span]], 1)
+        a = torch.cat([a[:, :span], a[:, span:] * a[:, :-span]], 1)
+        span *= 2
+    states = b + a * initial[:, None]
+    last = states[:, -1]
+    return (states.flip(1) if reverse else states), last
+
+
+def _run_recurrence(state, case):
+    gate, initial, reverse = state["gate"], state["initial"], case["reverse"]
+    if not case["backward"]:
+        if own:
+            ops, ws = _kept()
+            states, last = ops.linear_recurrence(ws, gate, state["value"], initial,
+                                                 reverse=reverse)
+        else:
+            states, last = _recur(gate.float(), state["value"].float(), initial, reverse)
+            states = states.to(gate.dtype)
+        return {"states": states, "last": last}
+    states, dstates, dlast = state["states"], state["dstates"], state["dlast"]
+    if own:
+        ops, ws = _kept()
+        dgate, dvalue, dinitial = ops.linear_recurrence_backward(
+            ws, gate, states, dstates, initial, dlast=dlast, reverse=reverse)
+        return {"dgate": dgate, "dvalue": dvalue, "dinitial": dinitial}
+    a = gate.float()
+    one = torch.ones_like(a[:, :1])
+    first, s = initial[:, None], states.float()
+    # The gradient runs against the recurrence, through the gate of the step after.
+    if reverse:
+        after, before = torch.cat([one, a[:, :-1]], 1), torch.cat([s[:, 1:], first], 1)
+    else:
+        after, before = torch.cat([a[:, 1:], one], 1), torch.cat([first, s[:, :-1]], 1)
+    g, end = _recur(after, dstates.float(), dlast, not reverse)
+    at = -1 if reverse else 0
+    return {"dgate": (g * before).to(gate.dtype), "dvalue": g.to(gate.dtype),
+            "dinitial": end * a[:, at]}
+
+
+# ---------------------------------------------------------------------------
+# What a pass cannot do without
+# ---------------------------------------------------------------------------
+def work(case):
+    size = {"float32": 4, "bfloat16": 2, "float16": 2}[case["dtype"]]
+    if case["kind"] == "recurrence":
+        n = case["batch"] * case["time"] * case["channels"]
+        ends = 4 * case["batch"] * case["channels"]
+        return {"bytes": n * size * (5 if case["backward"] else 3) + 2 * ends,
+                "flops": n * (3 if case["backward"] else 2)}
+    n, cells = case["rows"], case["rows"] * case["classes"]
+    passes = 1 + bool(case.get("backward") or case["kind"] != "logprobs")
+    size *= passes
+    if case.get("hessian"):
+        size += 4
+    if case["kind"] == "logprobs":
+        row = 8 + 4 * (1 + case["entropy"]) * passes
+    elif case["kind"] == "policy":
+        row = 8 + 4 * 4 + 4 * 4
+    else:
+        row = 8 + 4 + 4
+    pairs = case.get("pairs", 0)
+    return {"bytes": cells * size + n * row + pairs * 24, "flops": cells * (4 + 4 * (passes - 1))}
+
+
+# ---------------------------------------------------------------------------
+# The definitions, in 64 bits
+# ---------------------------------------------------------------------------
+def exact(case, seed):
+    s = prepare(case, seed)
+
+    def in_order(gate, value, initial):
+        """h_t = gate_t h_(t-1) + value_t step by step, over blocks of about sqrt(time) steps:
+        every block from a zero state first, then from the state that the block before leaves."""
+        b, t, c = gate.shape
+        block = max(1, math.isqrt(t))
+        blocks = -(-t // block)
+        pad = (0, 0, 0, blocks * block - t)
+        a = torch.nn.functional.pad(gate, pad).view(b, blocks, block, c)
+        v = torch.nn.functional.pad(value, pad).view(b, blocks, block, c).clone()
+        through = torch.ones_like(a)
+        through[:, :, 0] = a[:, :, 0]
+        for i in range(1, block):
+            v[:, :, i] += a[:, :, i] * v[:, :, i - 1]
+            through[:, :, i] = a[:, :, i] * through[:, :, i - 1]
+        start = torch.empty((b, blocks, c), dtype=torch.float64, device=gate.device)
+        h = initial
+        for j in range(blocks):
+            start[:, j] = h
+            h = v[:, j, -1] + through[:, j, -1] * h
+        return (v + through * start[:, :, None]).view(b, blocks * block, c)[:, :t]
+
+    if case["kind"] == "recurrence":
+        gate = s["gate"].double()
+        initial = s["initial"].double()
+        if case["reverse"]:
+            gate = gate.flip(1)
+        if not case["backward"]:
+            value = s["value"].double()
+            h = in_order(gate, value.flip(1) if case["reverse"] else value, initial)
+            return {"states": h.flip(1) if case["reverse"] else h, "last": h[:, -1]}
+        h, dh = s["states"].double(), s["dstates"].double()
+        if case["reverse"]:
+            h, dh = h.flip(1), dh.flip(1)
+        h = torch.cat([initial[:, None], h], 1)
+        dh[:, -1] += s["dlast"].double()
+        b, t, c = gate.shape
+        back = torch.zeros_like(gate)
+        back[:, 1:] = gate[:, 1:].flip(1)
+        g = in_order(back, dh.flip(1), torch.zeros_like(initial)).flip(1)
+        dgate = g * h[:, :-1]
+        end = g[:, 0] * gate[:, 0]
+        if case["reverse"]:
+            g, dgate = g.flip(1), dgate.flip(1)
+        return {"dgate": dgate, "dvalue": g, "dinitial": end}
+    action, n = s["action"], case["rows"]
+    kept = s["weight"] != 0 if case["kind"] == "policy" else action >= 0
+    rows = torch.arange(n, device=DEVICE)[kept]
+    y = action[rows]
+    lp = torch.log_softmax(s["margin"][rows].double(), 1)
+    p = lp.exp()
+    logp = lp.gather(1, y[:, None])[:, 0]
+    entropy = torch.special.entr(p).sum(1)
+
+    def whole(v):
+        return torch.zeros((n, *v.shape[1:]), dtype=torch.float64, device=DEVICE).index_copy_(
+            0, rows, v)
+
+    def through(dlogp, dentropy):
+        """p (v - p.v) with v the loss's gradient by the probabilities."""
+        v = -dentropy[:, None] * lp.clamp(min=-1e300)
+        v.scatter_add_(1, y[:, None], (dlogp / logp.exp())[:, None])
+        v.mul_(p)
+        return v.sub_(p * v.sum(1, keepdim=True))
+
+    def curvature(c):
+        return torch.maximum(2 * c[:, None] * (p - p * p),
+                             torch.tensor(1e-16, dtype=torch.float64, device=DEVICE))
+
+    if case["kind"] == "logprobs":
+        zero = torch.zeros_like(logp)
+        out = {"logp": whole(logp), "entropy": whole(entropy) if case["entropy"] else None}
+        if case["backward"]:
+            out["grad"] = whole(through(s["dlogp"][rows].double(),
+                                        s["dentropy"][rows].double() if case["entropy"] else zero))
+        return out
+    if case["kind"] == "policy":
+        w, adv = s["weight"][rows].double(), s["advantage"][rows].double()
+        ratio = (logp - s["old_logp"][rows].double()).exp()
+        lo, hi = 1 - case["clip_low"], 1 + case["clip_high"]
+        plain, cut = ratio * adv, ratio.clamp(lo, hi) * adv
+        d = s["reference"][rows].double() - logp
+        kl = d.exp() - 1 - d
+        loss = w * (case["kl"] * kl - case["entropy"] * entropy - torch.minimum(plain, cut))
+        free = (ratio < hi) & (adv > 0) | (ratio > lo) & (adv <= 0)
+        c = w * (case["kl"] * (1 - d.exp()) - plain * free)
+        grad = through(c, -case["entropy"] * w)
+        out = {"loss": loss, "logp": logp, "kl": kl, "entropy": entropy, "grad": grad,
+               "hess": curvature(c.abs() + case["entropy"] * w) if case["hessian"] else None}
+        return {k: None if v is None else whole(v) for k, v in out.items()}
+    ptr = s["sequences"]
+    seq = torch.searchsorted(ptr, rows, right=True) - 1
+    zero = torch.zeros(2 * case["pairs"], dtype=torch.float64, device=DEVICE)
+    total = zero.index_add(0, seq, logp - s["reference"][rows].double())
+    if case["average"]:
+        count = zero.index_add(0, seq, torch.ones_like(logp)).clamp(min=1)
+    else:
+        count = torch.ones_like(zero)
+    mean = (total / count).view(-1, 2)
+    score = case["beta"] * (mean[:, 0] - mean[:, 1])
+    e, good = case["smoothing"], torch.nn.functional.logsigmoid
+    slope = case["beta"] * (e * torch.sigmoid(score) - (1 - e) * torch.sigmoid(-score))
+    c = (torch.stack([slope, -slope], 1).view(-1) / count)[seq]
+    return {"loss": -(1 - e) * good(score) - e * good(-score), "score": score,
+            "logp": whole(logp), "grad": whole(through(c, torch.zeros_like(c))),
+            "hess": whole(curvature(c.abs())) if case["hessian"] else None}
