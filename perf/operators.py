@@ -274,7 +274,7 @@ def _run_policy(state, case):
     # The ratio is clipped where it passes the border on the advantage's side.  Rows that 32
     # bits cannot decide are looked at in 64.
     high, low = math.log1p(case["clip_high"]), math.log1p(-case["clip_low"])
-    border = torch.where(adv > 0, high, low)
+    border = torch.where(adv > 0, torch.full_like(logp, high), low)
     gap = logp - old.double() - border
     near = ((gap.abs() < 1e-5) & counted).nonzero()[:, 0]
     some = z[near].double()
