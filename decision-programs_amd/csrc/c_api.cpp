@@ -13,6 +13,7 @@
 
 #include "booster.hpp"
 #include "json.hpp"
+#include "policy.hpp"
 #include "tune.hpp"
 
 namespace dp {
@@ -111,6 +112,15 @@ void require_device_array(uintptr_t p, size_t bytes, const char* what) {
                " bytes from the pointer exceed its device allocation");
 }
 
+// A workspace whose scratch is on the current device.
+void require_workspace(dp_workspace ws) {
+  dp::need(ws != nullptr, "null workspace");
+  int device = 0;
+  DP_HIP(hipGetDevice(&device));
+  dp::need(ws->device == device, "the workspace belongs to device " + std::to_string(ws->device) +
+                                     ", not the current device " + std::to_string(device));
+}
+
 // Copies a float32 device array interface of shape [n] or [n, k] into dst.
 void copy_float_array(const ArrayInterface& a, int64_t n, int64_t k, float* dst) {
   dp::need(a.typestr == "<f4", "array interface must be little-endian float32 (<f4)");
@@ -184,6 +194,12 @@ void dp_workspace_s::reserve_scratch(size_t bytes) {
     while (cap < bytes) cap <<= 1;
     scratch.resize(cap);
   }
+}
+
+uint8_t* dp_workspace_s::scratch_only(size_t bytes) {
+  scratch_used = 0;
+  reserve_scratch(bytes);
+  return scratch.p;
 }
 
 void dp_workspace_s::need_scratch(size_t bytes) {
@@ -817,6 +833,97 @@ int dp_update_margin(dp_workspace ws, const uint32_t* ridx, const int64_t* begin
     std::copy(work.begin(), work.end(), ws->stage(work.size(), &d_work));
     ws->commit(s);
     dp::launch_update_margin(ridx, d_work, int32_t(work.size()), nullptr, margin, stride, s);
+  });
+}
+
+int dp_action_logprobs(dp_workspace ws, const dp_decisions* decisions, float* logp, float* entropy,
+                       void* stream) {
+  return guarded([&] {
+    require_workspace(ws);
+    dp::check_decisions(decisions);
+    if (decisions->n_rows == 0) return;
+    dp::need(logp != nullptr, "null argument");
+    dp::launch_action_logprobs(*decisions, logp, entropy, ws, as_stream(stream));
+  });
+}
+
+int dp_action_logprobs_backward(dp_workspace ws, const dp_decisions* decisions, const float* dlogp,
+                                const float* dentropy, void* grad, void* stream) {
+  return guarded([&] {
+    require_workspace(ws);
+    dp::check_decisions(decisions);
+    if (decisions->n_rows == 0) return;
+    dp::need(dlogp && grad, "null argument");
+    dp::launch_action_logprobs_backward(*decisions, dlogp, dentropy, grad, ws, as_stream(stream));
+  });
+}
+
+int dp_policy_loss(dp_workspace ws, const dp_decisions* decisions, const float* old_logp,
+                   const float* advantage, const float* weight, const float* reference,
+                   const dp_policy_param* param, float* loss, float* logp, float* kl,
+                   float* entropy, void* grad, float* hess, void* stream) {
+  return guarded([&] {
+    require_workspace(ws);
+    dp::check_decisions(decisions);
+    dp::need(param != nullptr, "null argument");
+    dp::need(param->clip_low >= 0.0 && param->clip_low <= 1.0 && param->clip_high >= 0.0 &&
+                 std::isfinite(param->clip_high),
+             "clip_low must be in [0, 1] and clip_high finite and nonnegative");
+    dp::need(param->kl >= 0.0 && std::isfinite(param->kl) && param->entropy >= 0.0 &&
+                 std::isfinite(param->entropy),
+             "kl and entropy weights must be finite and nonnegative");
+    dp::need(reference || (param->kl == 0.0 && !kl), "the KL term needs reference log-probabilities");
+    dp::need(!hess || (grad && decisions->dtype == DP_FLOAT32),
+             "hessians need float32 margins and a gradient");
+    if (decisions->n_rows == 0) return;
+    dp::need(old_logp && advantage && loss, "null argument");
+    dp::launch_policy_loss(*decisions, old_logp, advantage, weight, reference, *param, loss, logp,
+                           kl, entropy, grad, hess, ws, as_stream(stream));
+  });
+}
+
+int dp_preference_loss(dp_workspace ws, const dp_decisions* decisions, const int64_t* sequences,
+                       int64_t n_pairs, const float* reference, const dp_preference_param* param,
+                       float* loss, float* score, float* logp, void* grad, float* hess,
+                       void* stream) {
+  return guarded([&] {
+    require_workspace(ws);
+    dp::check_decisions(decisions);
+    dp::need(param != nullptr, "null argument");
+    dp::need(n_pairs >= 0 && n_pairs <= INT32_MAX, "pair count out of range");
+    dp::need(param->beta > 0.0 && std::isfinite(param->beta), "beta must be finite and positive");
+    dp::need(param->smoothing >= 0.0 && param->smoothing <= 1.0, "smoothing must be in [0, 1]");
+    dp::need(!hess || (grad && decisions->dtype == DP_FLOAT32),
+             "hessians need float32 margins and a gradient");
+    dp::need(n_pairs == 0 || (sequences && loss), "null argument");
+    dp::launch_preference_loss(*decisions, sequences, n_pairs, reference, *param, loss, score,
+                               logp, grad, hess, ws, as_stream(stream));
+  });
+}
+
+int dp_linear_recurrence(dp_workspace ws, const dp_recurrence* shape, const void* gate,
+                         const void* value, const float* initial, void* state, float* last,
+                         void* stream) {
+  return guarded([&] {
+    require_workspace(ws);
+    dp::check_recurrence(shape, 3);
+    if (shape->batch == 0 || shape->channels == 0) return;
+    dp::need(shape->time == 0 || (gate && value && state), "null argument");
+    dp::launch_recurrence(*shape, gate, value, initial, state, last, ws, as_stream(stream));
+  });
+}
+
+int dp_linear_recurrence_backward(dp_workspace ws, const dp_recurrence* shape, const void* gate,
+                                  const void* state, const void* dstate, const float* initial,
+                                  const float* dlast, void* dgate, void* dvalue, float* dinitial,
+                                  void* stream) {
+  return guarded([&] {
+    require_workspace(ws);
+    dp::check_recurrence(shape, 5);
+    if (shape->batch == 0 || shape->channels == 0) return;
+    dp::need(shape->time == 0 || (gate && state && dstate && dgate && dvalue), "null argument");
+    dp::launch_recurrence_backward(*shape, gate, state, dstate, initial, dlast, dgate, dvalue,
+                                   dinitial, ws, as_stream(stream));
   });
 }
 

@@ -273,6 +273,10 @@ struct dp_workspace_s {
     return reinterpret_cast<T*>(scratch.p + offset);
   }
   void reserve_scratch(size_t bytes);
+  // Device-only scratch for a call that stages nothing: no host wait and no
+  // event, so that a call whose scratch is large enough already can be captured
+  // into a graph.
+  uint8_t* scratch_only(size_t bytes);
 
  private:
   std::vector<uint8_t> committed_;  // the bytes the device staging area holds

@@ -7,8 +7,8 @@ Two layers mirror the two layers of ``include/dpgbdt.h``:
   device array interface, set labels, create a booster, set parameters,
   ``update(iter)``, save the model JSON.
 * ``ops``: the kernel-level operators (histogram, subtraction, split
-  evaluation, partition, gradients, quantisation, cuts, binning), taking torch
-  device tensors.
+  evaluation, partition, gradients, quantisation, cuts, binning, policy and
+  preference losses, linear recurrences), taking torch device tensors.
 
 torch is used only to own device memory and name streams.  There is no CPU
 fallback: loading fails loudly when the HIP library has not been built.
@@ -47,6 +47,27 @@ class SplitRecord(Structure):
     _fields_ = [("loss_chg", c_double), ("gl", c_int64), ("hl", c_int64), ("feature", c_int32),
                 ("bin", c_int32), ("default_left", c_int32), ("valid", c_int32),
                 ("expand", c_int32), ("pad", c_int32)]
+
+
+class Decisions(Structure):
+    _fields_ = [("margin", c_void_p), ("action", c_void_p), ("n_rows", c_int64),
+                ("row_stride", c_int64), ("n_classes", c_int32), ("dtype", c_int32),
+                ("action_bytes", c_int32), ("pad", c_int32)]
+
+
+class PolicyParam(Structure):
+    _fields_ = [("clip_low", c_double), ("clip_high", c_double), ("kl", c_double),
+                ("entropy", c_double)]
+
+
+class PreferenceParam(Structure):
+    _fields_ = [("beta", c_double), ("smoothing", c_double), ("average", c_int32),
+                ("pad", c_int32)]
+
+
+class Recurrence(Structure):
+    _fields_ = [("batch", c_int64), ("time", c_int64), ("channels", c_int64), ("dtype", c_int32),
+                ("reverse", c_int32), ("strides", (c_int64 * 2) * 5)]
 
 
 class TreeView(Structure):
@@ -147,6 +168,20 @@ def load():
                                  c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
         "dp_update_margin": (c_int, [H, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
                                      c_void_p, c_int64, c_void_p]),
+        "dp_action_logprobs": (c_int, [H, POINTER(Decisions), c_void_p, c_void_p, c_void_p]),
+        "dp_action_logprobs_backward": (c_int, [H, POINTER(Decisions), c_void_p, c_void_p,
+                                                c_void_p, c_void_p]),
+        "dp_policy_loss": (c_int, [H, POINTER(Decisions), c_void_p, c_void_p, c_void_p, c_void_p,
+                                   POINTER(PolicyParam), c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p]),
+        "dp_preference_loss": (c_int, [H, POINTER(Decisions), c_void_p, c_int64, c_void_p,
+                                       POINTER(PreferenceParam), c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_void_p]),
+        "dp_linear_recurrence": (c_int, [H, POINTER(Recurrence), c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_void_p]),
+        "dp_linear_recurrence_backward": (c_int, [H, POINTER(Recurrence), c_void_p, c_void_p,
+                                                  c_void_p, c_void_p, c_void_p, c_void_p,
+                                                  c_void_p, c_void_p, c_void_p]),
         "dp_synth": (c_int, [c_int32, c_uint64, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                              c_void_p, c_void_p]),
     }

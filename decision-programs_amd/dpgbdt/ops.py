@@ -6,12 +6,14 @@ torch.cuda.Event timing and ordering with torch work as usual.  Host arrays
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 from ctypes import c_int32, c_void_p
 
 import numpy as np
 
-from . import BinLayout, SplitRecord, TrainParam, check, load
+from . import BinLayout, Decisions, DPError, PolicyParam, PreferenceParam, Recurrence
+from . import SplitRecord, TrainParam, check, load
 
 SPLIT_DTYPE = np.dtype([("loss_chg", "<f8"), ("gl", "<i8"), ("hl", "<i8"), ("feature", "<i4"),
                         ("bin", "<i4"), ("default_left", "<i4"), ("valid", "<i4"),
@@ -244,3 +246,218 @@ def synth(config, n_rows, seed, device="cuda", n_features=None, want_grad=False)
     check(load().dp_synth(config, seed, n_rows, f, _ptr(values), _ptr(labels), _ptr(grad),
                           _ptr(hess), _stream()))
     return values, labels, grad, hess
+
+
+# ---------------------------------------------------------------------------
+# Decisions: policy and preference losses, advantages
+# ---------------------------------------------------------------------------
+PolicyLoss = collections.namedtuple("PolicyLoss", "loss logp kl entropy grad hess")
+PreferenceLoss = collections.namedtuple("PreferenceLoss", "loss score logp grad hess")
+
+
+def _need(ok, message):
+    if not ok:
+        raise DPError(message)
+
+
+def _dtype(t, what):
+    import torch
+
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+    _need(code is not None, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def _like(t, first, shape, what):
+    """Checks a float32 array that goes with the tensor `first`."""
+    import torch
+
+    _need(t.dtype is torch.float32 and t.shape == shape and t.is_contiguous()
+          and t.device == first.device,
+          f"{what} must be a contiguous float32 tensor of shape {tuple(shape)} on {first.device}")
+    return t
+
+
+def _on_current_device(t, what):
+    import torch
+
+    _need(t.is_cuda and t.get_device() == torch.cuda.current_device(),
+          f"{what} must be on the current device")
+
+
+def _decisions(margin, action):
+    import torch
+
+    _need(margin.dim() == 2, "margin must have shape [rows, classes]")
+    _on_current_device(margin, "margin")
+    n, k = margin.shape
+    _need(k >= 1, "margin must have at least one class")
+    _need(margin.stride(1) == 1 or k == 1, "the classes of a row must be adjacent")
+    _need(action.dtype in (torch.int64, torch.int32) and action.shape == (n,)
+          and action.is_contiguous() and action.device == margin.device,
+          f"action must be a contiguous int64 or int32 tensor of shape ({n},) on {margin.device}")
+    return Decisions(margin.data_ptr(), action.data_ptr(), n, margin.stride(0), k,
+                     _dtype(margin, "margin"), action.element_size())
+
+
+def action_logprobs(ws, margin, action, entropy=False):
+    """Log-probability of the action of every row of margins [n, K] (float32, float16 or
+    bfloat16; rows may be strided) -> (logp [n] float32, entropy [n] float32 or None).
+
+    Rows whose action is outside [0, K), or whose margins are all -infinity, are not counted: 0
+    for both."""
+    import torch
+
+    d = _decisions(margin, action)
+    logp = torch.empty(d.n_rows, dtype=torch.float32, device=margin.device)
+    h = torch.empty_like(logp) if entropy else None
+    check(load().dp_action_logprobs(ws.handle, ctypes.byref(d), _ptr(logp), _ptr(h), _stream()))
+    return logp, h
+
+
+def action_logprobs_backward(ws, margin, action, dlogp, dentropy=None):
+    """Gradient of the margins (their dtype, [n, K]) from those of action_logprobs' outputs."""
+    import torch
+
+    d = _decisions(margin, action)
+    _like(dlogp, margin, action.shape, "dlogp")
+    if dentropy is not None:
+        _like(dentropy, margin, action.shape, "dentropy")
+    grad = torch.empty(margin.shape, dtype=margin.dtype, device=margin.device)
+    check(load().dp_action_logprobs_backward(ws.handle, ctypes.byref(d), _ptr(dlogp),
+                                             _ptr(dentropy), _ptr(grad), _stream()))
+    return grad
+
+
+def policy_loss(ws, margin, action, old_logp, advantage, weight=None, reference=None,
+                clip_low=0.2, clip_high=0.2, kl=0.0, entropy=0.0, gradient=True, hessian=False):
+    """Clipped policy loss of every row, with a KL term to the policy whose log-probabilities of
+    the actions are `reference` and an entropy bonus, and its gradient of the margins
+    -> PolicyLoss(loss, logp, kl, entropy, grad, hess).
+
+    old_logp, advantage, weight and reference are float32 [n]; loss [n] holds the weighted rows,
+    so its sum is what grad [n, K] is the gradient of.  hess (float32 margins only) is what
+    Booster.boost takes beside grad.  kl is None without a reference, grad without gradient."""
+    import torch
+
+    d = _decisions(margin, action)
+    _like(old_logp, margin, action.shape, "old_logp")
+    _like(advantage, margin, action.shape, "advantage")
+    if weight is not None:
+        _like(weight, margin, action.shape, "weight")
+    if reference is not None:
+        _like(reference, margin, action.shape, "reference")
+    _need(gradient or not hessian, "a hessian needs the gradient")
+    out = torch.empty((4, d.n_rows), dtype=torch.float32, device=margin.device)
+    loss, logp, k, h = out.unbind()
+    k = k if reference is not None else None
+    grad = (torch.empty(margin.shape, dtype=margin.dtype, device=margin.device)
+            if gradient else None)
+    hess = (torch.empty(margin.shape, dtype=torch.float32, device=margin.device)
+            if hessian else None)
+    param = PolicyParam(clip_low, clip_high, kl, entropy)
+    check(load().dp_policy_loss(ws.handle, ctypes.byref(d), _ptr(old_logp), _ptr(advantage),
+                                _ptr(weight), _ptr(reference), ctypes.byref(param), _ptr(loss),
+                                _ptr(logp), _ptr(k), _ptr(h), _ptr(grad), _ptr(hess), _stream()))
+    return PolicyLoss(loss, logp, k, h, grad, hess)
+
+
+def preference_loss(ws, margin, action, sequences, reference=None, beta=0.1, smoothing=0.0,
+                    average=False, gradient=True, hessian=False):
+    """Preference loss of pairs of row sequences and its gradient of the margins
+    -> PreferenceLoss(loss [P], score [P], logp [n], grad [n, K], hess).
+
+    sequences (int64 [2 P + 1], on the device) holds the offsets of the sequences' rows; pair i
+    prefers sequence 2 i to sequence 2 i + 1.  reference (float32 [n]) holds the reference
+    policy's log-probabilities of the actions; loss.sum() is what grad is the gradient of."""
+    import torch
+
+    d = _decisions(margin, action)
+    _need(sequences.dtype is torch.int64 and sequences.dim() == 1 and sequences.is_contiguous()
+          and len(sequences) % 2 == 1 and sequences.device == margin.device,
+          f"sequences must be a contiguous int64 tensor of 2 P + 1 offsets on {margin.device}")
+    if reference is not None:
+        _like(reference, margin, action.shape, "reference")
+    _need(gradient or not hessian, "a hessian needs the gradient")
+    pairs = len(sequences) // 2
+    dev = margin.device
+    loss = torch.empty(pairs, dtype=torch.float32, device=dev)
+    score = torch.empty_like(loss)
+    logp = torch.empty(d.n_rows, dtype=torch.float32, device=dev)
+    grad = torch.empty(margin.shape, dtype=margin.dtype, device=dev) if gradient else None
+    hess = torch.empty(margin.shape, dtype=torch.float32, device=dev) if hessian else None
+    param = PreferenceParam(beta, smoothing, bool(average))
+    check(load().dp_preference_loss(ws.handle, ctypes.byref(d), _ptr(sequences), pairs,
+                                    _ptr(reference), ctypes.byref(param), _ptr(loss), _ptr(score),
+                                    _ptr(logp), _ptr(grad), _ptr(hess), _stream()))
+    return PreferenceLoss(loss, score, logp, grad, hess)
+
+
+def _recurrence(reverse, arrays, ends):
+    """The C description of [B, T, C] arrays and checks of the float32 [B, C] ones."""
+    import torch
+
+    first = arrays[0][0]
+    _need(first.dim() == 3, f"{arrays[0][1]} must have shape [batch, time, channels]")
+    _on_current_device(first, arrays[0][1])
+    b, t, c = first.shape
+    shape = Recurrence(b, t, c, _dtype(first, arrays[0][1]), bool(reverse))
+    for i, (x, what) in enumerate(arrays):
+        _need(x.dtype is first.dtype and x.shape == first.shape and x.device == first.device,
+              f"{what} must be {first.dtype} of shape {(b, t, c)} on {first.device}")
+        _need(c <= 1 or x.stride(2) == 1, f"the channels of {what} must be adjacent")
+        shape.strides[i][0], shape.strides[i][1] = x.stride(0), x.stride(1)
+    for x, what in ends:
+        if x is not None:
+            _like(x, first, torch.Size((b, c)), what)
+    return shape
+
+
+def _dense_like(x):
+    """An empty tensor in x's order of dimensions, without its gaps or repeats."""
+    import torch
+
+    out = torch.empty_like(x)  # keeps the strides of dense tensors only
+    return out if out.dim() != 3 or out.shape[2] <= 1 or out.stride(2) == 1 else out.contiguous()
+
+
+def linear_recurrence(ws, gate, value, initial=None, reverse=False):
+    """state_t = gate_t state_(t-1) + value_t over the time of [B, T, C] tensors (reverse: from
+    the state after) -> (state in value's dtype and order, last state [B, C] float32).
+
+    initial (float32 [B, C]) is the state before the first step, zero without.  Batch and time
+    may be strided (time-major arrays as a transposed view, a gate expanded over batch or time);
+    channels are adjacent.  With a single step (T = 1) and initial = last of the call before, it
+    is one step of a running recurrence.  Advantages: value the temporal differences, gate
+    gamma * lambda, 0 where an episode ends, reverse=True."""
+    import torch
+
+    shape = _recurrence(reverse, [(gate, "gate"), (value, "value")], [(initial, "initial")])
+    state = _dense_like(value)
+    shape.strides[2][0], shape.strides[2][1] = state.stride(0), state.stride(1)
+    last = torch.empty((shape.batch, shape.channels), dtype=torch.float32, device=gate.device)
+    check(load().dp_linear_recurrence(ws.handle, ctypes.byref(shape), _ptr(gate), _ptr(value),
+                                      _ptr(initial), _ptr(state), _ptr(last), _stream()))
+    return state, last
+
+
+def linear_recurrence_backward(ws, gate, state, dstate, initial=None, dlast=None, reverse=False):
+    """Gradients of linear_recurrence's inputs from those of its outputs (dlast: float32 [B, C],
+    zero without) and the states it returned -> (dgate, dvalue, dinitial [B, C] float32).
+
+    An input that was expanded has the sum of its gradient over the expanded dimension."""
+    import torch
+
+    shape = _recurrence(reverse, [(gate, "gate"), (state, "state"), (dstate, "dstate")],
+                        [(initial, "initial"), (dlast, "dlast")])
+    dvalue = _dense_like(dstate)
+    dgate = torch.empty_strided(dvalue.shape, dvalue.stride(), dtype=gate.dtype,
+                                device=gate.device)
+    for i, x in ((3, dgate), (4, dvalue)):
+        shape.strides[i][0], shape.strides[i][1] = x.stride(0), x.stride(1)
+    dinitial = torch.empty((shape.batch, shape.channels), dtype=torch.float32, device=gate.device)
+    check(load().dp_linear_recurrence_backward(ws.handle, ctypes.byref(shape), _ptr(gate),
+                                               _ptr(state), _ptr(dstate), _ptr(initial),
+                                               _ptr(dlast), _ptr(dgate), _ptr(dvalue),
+                                               _ptr(dinitial), _stream()))
+    return dgate, dvalue, dinitial

@@ -369,6 +369,113 @@ int dp_update_margin(dp_workspace ws, const uint32_t* ridx, const int64_t* begin
                      const int64_t* end, const float* value, int32_t n_leaves, float* margin,
                      int64_t stride, void* stream);
 
+/* ---- decisions: policy and preference losses, advantages --------------- */
+/* What training a policy needs around the booster: a model's margins over
+ * classes (logits) and the class taken in every row become losses and the
+ * gradients that XGBoosterTrainOneIter takes.  No counterpart in the reference.
+ * With n_classes logits a row, p = softmax(margin) and y the action of the row:
+ *   log p_y, entropy H = -sum p log p.
+ * A row whose action is outside [0, n_classes) or whose weight is 0 is not
+ * counted: its margins are not looked at (they may hold NaN), its outputs,
+ * gradient and hessian are 0.  A class whose margin is -infinity has probability
+ * 0 and gradient 0; a row with no other class is not counted either.  NaN in a counted row reaches that row's outputs only
+ * (and its pair's).  Sums and statistics are held in 32 bits or more, log p_y
+ * and its differences in 64; the same call gives the same bits every time.
+ * The calls allocate nothing once the workspace has grown to their size, and
+ * can be captured into a graph then. */
+enum dp_dtype { DP_FLOAT32 = 0, DP_FLOAT16 = 1, DP_BFLOAT16 = 2 };
+
+typedef struct {
+  const void* margin;   /* device [n_rows][n_classes] of dtype; row r at r * row_stride */
+  const void* action;   /* device [n_rows], int32 or int64 */
+  int64_t n_rows;
+  int64_t row_stride;   /* elements */
+  int32_t n_classes;
+  int32_t dtype;        /* dp_dtype */
+  int32_t action_bytes; /* 4 or 8 */
+  int32_t pad;
+} dp_decisions;
+
+/* logp [n_rows] = log p_y and, unless NULL, entropy [n_rows]. */
+int dp_action_logprobs(dp_workspace ws, const dp_decisions* decisions, float* logp, float* entropy,
+                       void* stream);
+
+/* grad [n_rows][n_classes] (dtype, dense): the margins' gradient of
+ * sum dlogp log p_y + dentropy H (dentropy NULL: 0). */
+int dp_action_logprobs_backward(dp_workspace ws, const dp_decisions* decisions, const float* dlogp,
+                                const float* dentropy, void* grad, void* stream);
+
+typedef struct {
+  double clip_low, clip_high; /* the ratio's bounds 1 - clip_low, 1 + clip_high */
+  double kl, entropy;         /* weights of the KL term and of the entropy bonus */
+} dp_policy_param;
+
+/* Clipped policy loss of every row, with ratio = exp(log p_y - old_logp),
+ * k = e^d - 1 - d, d = reference - log p_y (an unbiased estimate of the KL
+ * divergence from the reference policy, whose log-probabilities of the actions
+ * are `reference`):
+ *   loss = weight * (-min(ratio * advantage, clip(ratio) * advantage)
+ *                    + kl * k - entropy * H)
+ * logp = log p_y, kl = k and entropy = H come without the weight.  Which side
+ * of the clip's border a ratio is on is decided as in 64 bits.  Gradient
+ * c ([k == y] - p_k) + n p_k (log p_k + H) with c the loss's slope by log p_y and
+ * n = weight * entropy; hessian max(2 (|c| + |n|) p_k (1 - p_k), 1e-16).
+ * weight NULL: 1.  reference may be NULL when param->kl is 0 and kl is NULL.
+ * logp, kl, entropy, grad and hess may be NULL; hess needs grad and DP_FLOAT32. */
+int dp_policy_loss(dp_workspace ws, const dp_decisions* decisions, const float* old_logp,
+                   const float* advantage, const float* weight, const float* reference,
+                   const dp_policy_param* param, float* loss, float* logp, float* kl,
+                   float* entropy, void* grad, float* hess, void* stream);
+
+typedef struct {
+  double beta, smoothing; /* scale of the scores; share of pairs that are the wrong way round */
+  int32_t average;        /* 1: means over a sequence's counted rows instead of sums */
+  int32_t pad;
+} dp_preference_param;
+
+/* Preference loss of every pair of row sequences: pair i prefers sequence 2 i
+ * (rows sequences[2 i] .. sequences[2 i + 1] - 1) to sequence 2 i + 1.  sequences
+ * (device, 2 n_pairs + 1 offsets) must not decrease; offsets are cut to
+ * [0, n_rows].  S of a sequence is the sum of log p_y - reference over its
+ * counted rows (reference NULL: 0), in 64 bits:
+ *   score = beta (S of 2 i - S of 2 i + 1)
+ *   loss = -(1 - smoothing) log sigma(score) - smoothing log sigma(-score)
+ * logp [n_rows], score [n_pairs], grad and hess as in dp_policy_loss (rows of no
+ * sequence: 0); all four may be NULL. */
+int dp_preference_loss(dp_workspace ws, const dp_decisions* decisions, const int64_t* sequences,
+                       int64_t n_pairs, const float* reference, const dp_preference_param* param,
+                       float* loss, float* score, float* logp, void* grad, float* hess,
+                       void* stream);
+
+/* Gated linear recurrence over the time of [batch][time][channels] arrays:
+ * state_t = gate_t * state_(t-1) + value_t; with reverse, state_t = gate_t *
+ * state_(t+1) + value_t (advantages: value the temporal differences, gate
+ * gamma * lambda where the episode goes on and 0 where it ends).  Element
+ * (b, t, c) of array i is at b * strides[i][0] + t * strides[i][1] + c.  States
+ * are held in 32 bits.  Products of gates over a span are formed, so they must
+ * not overflow (gates of at most 1 in size never do). */
+typedef struct {
+  int64_t batch, time, channels;
+  int32_t dtype;   /* dp_dtype of all arrays but initial, last, dlast, dinitial (float) */
+  int32_t reverse;
+  int64_t strides[5][2]; /* elements: batch, time */
+} dp_recurrence;
+
+/* strides: gate, value, state.  initial [batch][channels] (NULL: 0) is the state
+ * before the first step, last [batch][channels] (NULL: not wanted) the one after
+ * the last step. */
+int dp_linear_recurrence(dp_workspace ws, const dp_recurrence* shape, const void* gate,
+                         const void* value, const float* initial, void* state, float* last,
+                         void* stream);
+
+/* Gradients from those of the states (dstate) and of last (dlast, NULL: 0), with
+ * the states that the forward call left.  strides: gate, state, dstate, dgate,
+ * dvalue.  dinitial may be NULL. */
+int dp_linear_recurrence_backward(dp_workspace ws, const dp_recurrence* shape, const void* gate,
+                                  const void* state, const void* dstate, const float* initial,
+                                  const float* dlast, void* dgate, void* dvalue, float* dinitial,
+                                  void* stream);
+
 /* ---- synthetic workloads (benchmark inputs; not part of the path) ------ */
 /* config 1..5 as listed in the benchmark definition; writes values
  * [n_rows][n_features], labels [n_rows] and, for config 3, grad/hess [n_rows]
