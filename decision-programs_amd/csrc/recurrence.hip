@@ -2,84 +2,400 @@
 // [channels] arrays, in either direction of time, and its gradients.
 //
 // The gradient of the states runs against the recurrence: with g_t the whole
-// gradient of h_t, g_t = dh_t + a_(t+1) g_(t+1) (beyond the end: the last state's
-// own gradient, through a gate of 1), db_t = g_t, da_t = g_t h_(t-1) and
-// dh_0 = a_1 g_1.  So both passes are one scan: forward x_t = b_t with gate a_t,
-// backward x_t = dh_t with the gate of the step before it in its own direction.
+// gradient of h_t, g_t = dh_t + c_(t+1), c_t = a_t g_t (beyond the end, c is the last
+// state's own gradient), db_t = g_t, da_t = g_t h_(t-1) and dh_0 = c_1.  So both
+// passes are one scan, of h or of c: a step is h -> a h + b forward and
+// c -> a (dh + c) backward, and steps join as pairs (A, B): x -> A x + B.
+//
+// A lane takes kSteps neighbouring steps of its columns into registers and joins
+// them; the lanes of a wave, then its workgroup's waves, join theirs; with the state
+// before them the steps are taken again, from the registers, and stored.  So the
+// arrays are read once.  A workgroup goes on to the next steps with the state that
+// these leave.  Where the columns do not fill the chip, time is split over
+// workgroups: one launch joins each split's steps, the next starts from the splits
+// before, and both gate and values are read twice.
 //
 // States are held in 32 bits and rounded once where they are stored in 16.
 #include <algorithm>
+#include <bit>
+#include <type_traits>
 
 #include "policy.hpp"
 
 namespace dp {
 namespace {
 
-constexpr int kScanThreads = 256;
+constexpr int kMostWaves = 16;
 
 struct Strides {
   int64_t batch, time;
 };
 
+// Arrays of [batch][time][channels]; in the scan's own direction, step k is time k, or
+// time - 1 - k with down.  A column is a channel of a batch's.
 struct Scan {
-  int64_t batch, time;
-  int32_t channels;
-  bool down;  // time runs down in the scan's own direction
+  int64_t batch, time, channels;
+  bool down;
+  int32_t lanes;       // of a wave side by side over columns: 1 to 64
+  int32_t splits;      // of time, each of split_steps
+  int64_t batch_lanes; // over the channels of a batch
+  int64_t first, groups;  // of lanes, one a workgroup: the launch's
+  int64_t split_steps;
   const void *gate, *x, *state;
   const float *initial, *carry;  // of the recurrence; the scan's start (null: zero)
   void *out, *dgate;
   float* end;
+  float* sums;  // [splits][2][batch][channels]: A, B
   Strides gate_at, x_at, state_at, out_at, dgate_at;
 };
 
-// A thread a channel, step by step.
-template <class T, bool BACK>
-__global__ __launch_bounds__(kScanThreads) void scan_kernel(Scan a) {
-  const int64_t lanes = a.batch * a.channels;
-  for (int64_t i = int64_t(blockIdx.x) * kScanThreads + threadIdx.x; i < lanes;
-       i += int64_t(gridDim.x) * kScanThreads) {
-    const int64_t b = i / a.channels, c = i - b * a.channels;
-    const T* gate = static_cast<const T*>(a.gate) + b * a.gate_at.batch + c;
-    const T* x = static_cast<const T*>(a.x) + b * a.x_at.batch + c;
-    const T* state = BACK ? static_cast<const T*>(a.state) + b * a.state_at.batch + c : nullptr;
-    T* out = static_cast<T*>(a.out) + b * a.out_at.batch + c;
-    T* dgate = BACK ? static_cast<T*>(a.dgate) + b * a.dgate_at.batch + c : nullptr;
-    float h = a.carry ? a.carry[i] : 0.0f;
-    float before = 1.0f;  // BACK: the gate of the step before
-    for (int64_t k = 0; k < a.time; ++k) {
-      const int64_t t = a.down ? a.time - 1 - k : k;
-      const float g = float(gate[t * a.gate_at.time]);
-      h = fmaf(BACK ? before : g, h, float(x[t * a.x_at.time]));
-      out[t * a.out_at.time] = T(h);
-      if (BACK) {
-        const int64_t p = a.down ? t - 1 : t + 1;
-        const float hp = k + 1 < a.time ? float(state[p * a.state_at.time])
-                                        : (a.initial ? a.initial[i] : 0.0f);
-        dgate[t * a.dgate_at.time] = T(h * hp);
-        before = g;
+// Where a lane's columns of an array are, at step 0, and how far apart steps are.
+template <class T>
+struct Track {
+  T* p;
+  int64_t step;
+};
+
+template <class T, class P>
+__device__ __forceinline__ Track<T> track(const Scan& a, P* base, const Strides& at, int64_t batch,
+                                          int64_t channel) {
+  T* p = static_cast<T*>(base) + batch * at.batch + channel;
+  if (a.down) p += (a.time - 1) * at.time;
+  return {p, a.down ? -at.time : at.time};
+}
+
+// STEPS steps of one array in registers: WIDTH neighbouring columns a step, or, where steps
+// are neighbours (LINE: 1 up, -1 down), vectors of steps.
+template <class T, int STEPS, int WIDTH, int LINE>
+struct Steps {
+  static constexpr int kWords = LINE ? STEPS * int(sizeof(T)) / 4 : STEPS;
+  static constexpr int N = 16 / int(sizeof(T));
+  uint32_t w[kWords] = {};
+
+  static __device__ __forceinline__ float unpack(uint32_t w, int half) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w);
+    else if constexpr (std::is_same_v<T, __bf16>)
+      return __builtin_bit_cast(float, half ? w & 0xffff0000u : w << 16);
+    else return float(__builtin_bit_cast(T, uint16_t(half ? w >> 16 : w)));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, lo);
+    else {
+      typedef T Pair __attribute__((ext_vector_type(2)));
+      return __builtin_bit_cast(uint32_t, Pair{T(lo), T(hi)});
+    }
+  }
+  __device__ __forceinline__ float get(int s, int c) const {
+    if constexpr (LINE == 0) return unpack(w[s], c);
+    const int at = LINE > 0 ? s : STEPS - 1 - s;
+    if constexpr (sizeof(T) == 4) return unpack(w[at], 0);
+    return unpack(w[at / 2], at & 1);
+  }
+  __device__ __forceinline__ void set(int s, const float* v) {  // one step
+    if constexpr (LINE == 0) {
+      w[s] = pack(v[0], v[WIDTH - 1]);
+    } else {
+      const int at = LINE > 0 ? s : STEPS - 1 - s;
+      if constexpr (sizeof(T) == 4) w[at] = pack(v[0], v[0]);
+      else {
+        const uint32_t one = pack(v[0], 0.0f) & 0xffffu;
+        w[at / 2] = at & 1 ? (w[at / 2] & 0xffffu) | one << 16 : (w[at / 2] & 0xffff0000u) | one;
       }
     }
-    if (a.end) a.end[i] = BACK ? before * h : h;
+  }
+  // One step from memory.
+  __device__ __forceinline__ void load_one(int s, const T* p) {
+    if constexpr (LINE != 0) {
+      const float v[1] = {float(*p)};
+      set(s, v);
+    } else if constexpr (WIDTH * sizeof(T) == 4) {
+      __builtin_memcpy(&w[s], p, 4);
+    } else {
+      w[s] = __builtin_bit_cast(uint16_t, *p);
+    }
+  }
+  __device__ __forceinline__ void store_one(int s, T* p) const {
+    if constexpr (LINE != 0) *p = T(get(s, 0));
+    else if constexpr (WIDTH * sizeof(T) == 4) __builtin_memcpy(p, &w[s], 4);
+    else *p = __builtin_bit_cast(T, uint16_t(w[s]));
+  }
+  __device__ __forceinline__ void load_all(const Track<const T>& t, int64_t k) {
+    if constexpr (LINE != 0) {
+      const T* p = LINE > 0 ? t.p + k : t.p - k - (STEPS - 1);
+#pragma unroll
+      for (int i = 0; i < STEPS / N; ++i) __builtin_memcpy(w + 4 * i, p + i * N, 16);
+    } else {
+      const T* p = t.p + k * t.step;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s, p += t.step) load_one(s, p);
+    }
+  }
+  __device__ __forceinline__ void store_all(const Track<T>& t, int64_t k) const {
+    if constexpr (LINE != 0) {
+      T* p = LINE > 0 ? t.p + k : t.p - k - (STEPS - 1);
+#pragma unroll
+      for (int i = 0; i < STEPS / N; ++i) __builtin_memcpy(p + i * N, w + 4 * i, 16);
+    } else {
+      T* p = t.p + k * t.step;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s, p += t.step) store_one(s, p);
+    }
+  }
+};
+
+// SUMS: joins each split's steps only.
+template <class T, bool BACK, bool SUMS, int STEPS, int WIDTH, int LINE>
+__global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
+  using Kept = Steps<T, STEPS, WIDTH, LINE>;
+  __shared__ float joined[2][kMostWaves][2][64 * WIDTH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int across = lane & (a.lanes - 1), along = lane / a.lanes, depth = 64 / a.lanes;
+  const unsigned group = blockIdx.x % unsigned(a.groups), split = blockIdx.x / unsigned(a.groups);
+  int64_t index = (a.first + group) * a.lanes + across;
+  const bool live = index < a.batch * a.batch_lanes;
+  index = live ? index : 0;
+  const int64_t batch = a.batch * a.batch_lanes <= UINT32_MAX
+                            ? int64_t(uint32_t(index) / uint32_t(a.batch_lanes))
+                            : index / a.batch_lanes;
+  // An odd number of channels: the last ones twice, with the same results.
+  const int64_t channel =
+      min((index - batch * a.batch_lanes) * WIDTH, a.channels - int64_t(WIDTH));
+  const int64_t end_at = batch * a.channels + channel, all = a.batch * a.channels;
+
+  const auto gate = track<const T>(a, a.gate, a.gate_at, batch, channel);
+  const auto x = track<const T>(a, a.x, a.x_at, batch, channel);
+  const auto state = track<const T>(a, a.state, a.state_at, batch, channel);
+  const auto out = track<T>(a, a.out, a.out_at, batch, channel);
+  const auto dgate = track<T>(a, a.dgate, a.dgate_at, batch, channel);
+
+  const int64_t begin = int64_t(split) * a.split_steps, end = min(begin + a.split_steps, a.time);
+  float h[WIDTH], through[WIDTH], first[WIDTH];  // the state before the block; SUMS: A so far
+#pragma unroll
+  for (int c = 0; c < WIDTH; ++c) {
+    h[c] = !SUMS && a.carry && live ? a.carry[end_at + c] : 0.0f;
+    first[c] = BACK && !SUMS && a.initial && live ? a.initial[end_at + c] : 0.0f;
+    through[c] = 1.0f;
+  }
+  if (!SUMS && live)
+    for (unsigned i = 0; i < split; ++i) {
+      const float* at = a.sums + 2 * i * all + end_at;
+#pragma unroll
+      for (int c = 0; c < WIDTH; ++c) h[c] = fmaf(at[c], h[c], at[all + c]);
+    }
+
+  const int64_t block = int64_t(waves) * depth * STEPS;
+  int turn = 0;
+  for (int64_t k0 = begin; k0 < end; k0 += block, turn ^= 1) {
+    const int64_t k = k0 + int64_t(wave * depth + along) * STEPS;
+    // Whole: no step of the lane is outside, nor is the state that a backward step looks at.
+    const bool whole = live && k + STEPS <= end && (!BACK || k + STEPS < a.time);
+    const int count = !live ? 0 : int(min(max(end - k, int64_t(0)), int64_t(STEPS)));
+    Kept g, v, before;
+    if (whole) {
+      g.load_all(gate, k);
+      v.load_all(x, k);
+      if (BACK && !SUMS) before.load_all(state, k + 1);
+    } else {
+      // Steps outside keep the state.
+      const float one[2] = {1.0f, 1.0f}, zero[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        g.set(s, one);
+        v.set(s, zero);
+        if (BACK && !SUMS) before.set(s, zero);
+        if (s < count) {
+          g.load_one(s, gate.p + (k + s) * gate.step);
+          v.load_one(s, x.p + (k + s) * x.step);
+          if (BACK && !SUMS && k + s + 1 < a.time)
+            before.load_one(s, state.p + (k + s + 1) * state.step);
+        }
+      }
+    }
+    float A[WIDTH], B[WIDTH];
+#pragma unroll
+    for (int c = 0; c < WIDTH; ++c) {
+      A[c] = 1.0f;
+      B[c] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const float gate_s = g.get(s, c);
+        A[c] *= gate_s;
+        B[c] = BACK ? gate_s * (v.get(s, c) + B[c]) : fmaf(gate_s, B[c], v.get(s, c));
+      }
+      // with the lanes before
+      for (int d = a.lanes; d < 64; d <<= 1) {
+        const float A0 = __shfl_up(A[c], d, 64), B0 = __shfl_up(B[c], d, 64);
+        if (lane >= d) {
+          B[c] = fmaf(A[c], B0, B[c]);
+          A[c] *= A0;
+        }
+      }
+      if (along == depth - 1) {
+        joined[turn][wave][0][across * WIDTH + c] = A[c];
+        joined[turn][wave][1][across * WIDTH + c] = B[c];
+      }
+      // of the lanes before alone
+      const float A0 = __shfl_up(A[c], a.lanes, 64), B0 = __shfl_up(B[c], a.lanes, 64);
+      A[c] = along ? A0 : 1.0f;
+      B[c] = along ? B0 : 0.0f;
+    }
+    __syncthreads();
+    float mine[WIDTH];
+#pragma unroll
+    for (int c = 0; c < WIDTH; ++c) {
+      for (int w = 0; w < waves; ++w) {
+        if (w == wave) mine[c] = h[c];
+        const float Aw = joined[turn][w][0][across * WIDTH + c];
+        h[c] = fmaf(Aw, h[c], joined[turn][w][1][across * WIDTH + c]);
+        if (SUMS) through[c] *= Aw;
+      }
+      mine[c] = fmaf(A[c], mine[c], B[c]);
+    }
+    if (SUMS) continue;
+    Kept o, da;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      float y[WIDTH], d[WIDTH];
+#pragma unroll
+      for (int c = 0; c < WIDTH; ++c) {
+        if (BACK) {
+          y[c] = v.get(s, c) + mine[c];
+          const float hp = k + s + 1 == a.time ? first[c] : before.get(s, c);
+          d[c] = y[c] * hp;
+          mine[c] = g.get(s, c) * y[c];
+        } else {
+          mine[c] = y[c] = fmaf(g.get(s, c), mine[c], v.get(s, c));
+        }
+      }
+      o.set(s, y);
+      if (BACK) da.set(s, d);
+    }
+    if (whole) {
+      o.store_all(out, k);
+      if (BACK) da.store_all(dgate, k);
+    } else {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (s < count) {
+          o.store_one(s, out.p + (k + s) * out.step);
+          if (BACK) da.store_one(s, dgate.p + (k + s) * dgate.step);
+        }
+    }
+  }
+  if (wave != 0 || along != 0 || !live) return;
+#pragma unroll
+  for (int c = 0; c < WIDTH; ++c) {
+    if (SUMS) {
+      a.sums[2 * split * all + end_at + c] = through[c];
+      a.sums[(2 * split + 1) * all + end_at + c] = h[c];
+    } else if (a.end && int(split) == a.splits - 1) {
+      a.end[end_at + c] = h[c];
+    }
   }
 }
 
 template <bool BACK>
-void launch_scan(const Scan& a, int32_t dtype, hipStream_t s) {
-  const int64_t lanes = a.batch * a.channels;
-  if (lanes == 0) return;
-  const unsigned grid =
-      unsigned(std::min<int64_t>((lanes + kScanThreads - 1) / kScanThreads, 1 << 20));
-  with_element(dtype, [&](auto t) {
-    scan_kernel<decltype(t), BACK><<<grid, kScanThreads, 0, s>>>(a);
-  });
+constexpr int kSteps = BACK ? 8 : 16;
+
+template <class T, bool BACK, int WIDTH, int LINE>
+void launch_typed(Scan a, unsigned waves, hipStream_t s) {
+  constexpr int steps = kSteps<BACK>;
+  if (a.splits > 1) {
+    const unsigned n = unsigned(a.groups);
+    scan_kernel<T, BACK, true, steps, WIDTH, LINE>
+        <<<n * unsigned(a.splits - 1), waves * 64, 0, s>>>(a);
+    DP_HIP(hipGetLastError());
+    scan_kernel<T, BACK, false, steps, WIDTH, LINE>
+        <<<n * unsigned(a.splits), waves * 64, 0, s>>>(a);
+  } else {
+    // A launch has fewer than 2^32 threads.
+    const int64_t most = int64_t(1) << 21, groups = a.groups;
+    for (a.first = 0; a.first < groups; a.first += most) {
+      a.groups = std::min(groups - a.first, most);
+      scan_kernel<T, BACK, false, steps, WIDTH, LINE>
+          <<<unsigned(a.groups), waves * 64, 0, s>>>(a);
+    }
+  }
   DP_HIP(hipGetLastError());
+}
+
+int64_t cover(int64_t n, int64_t by) { return (n + by - 1) / by; }
+
+// How the scan lies on the chip.
+struct Plan {
+  Scan scan;
+  unsigned waves;  // of a workgroup
+  int line, width;
+};
+
+constexpr int64_t kWorkgroups = 512;  // that fill the chip
+constexpr int64_t kMostSplits = 64;
+
+template <bool BACK>
+Plan plan_of(Scan a, int element) {
+  Plan p{};
+  const Strides* at[] = {&a.gate_at, &a.x_at, &a.out_at, &a.state_at, &a.dgate_at};
+  bool merge = true, line = a.channels == 1;
+  for (int i = 0; i < (BACK ? 5 : 3); ++i) {
+    merge = merge && (a.batch == 1 || at[i]->batch == a.channels);
+    line = line && (a.time <= 1 || at[i]->time == 1);
+  }
+  line = line && (a.batch == 1 || !merge);
+  if (merge) {  // sequences side by side are channels
+    a.channels *= a.batch;
+    a.batch = 1;
+  }
+  p.line = !line ? 0 : a.down ? -1 : 1;
+  p.width = element == 2 && a.channels >= 2 ? 2 : 1;
+  a.batch_lanes = cover(a.channels, p.width);
+
+  const int64_t lanes = a.batch * a.batch_lanes;
+  const int64_t parts = cover(std::max<int64_t>(a.time, 1), kSteps<BACK>);
+  const int64_t needed = int64_t(std::bit_ceil(uint64_t(std::min<int64_t>(parts, 64))));
+  int64_t across;
+  if (line) {
+    across = 64 / needed;
+  } else {
+    across = int64_t(std::bit_ceil(uint64_t(std::min<int64_t>(lanes, 64))));
+    // Narrower groups while there are too few, down to 32 bytes a step.
+    while (across > 8 && cover(lanes, across) < kWorkgroups && needed > 64 / across) across /= 2;
+  }
+  a.lanes = int32_t(across);
+  a.groups = cover(lanes, across);
+  const int64_t depth = 64 / across;
+  p.waves = unsigned(std::min<uint64_t>(std::bit_ceil(uint64_t(cover(parts, depth))), kMostWaves));
+  const int64_t block = int64_t(p.waves) * depth * kSteps<BACK>;
+  const int64_t blocks = cover(std::max<int64_t>(a.time, 1), block);
+  int64_t splits = 1;
+  if (a.groups < kWorkgroups / 2)
+    splits = std::min({cover(kWorkgroups, a.groups), blocks, kMostSplits});
+  a.split_steps = cover(blocks, splits) * block;
+  a.splits = int32_t(cover(std::max<int64_t>(a.time, 1), a.split_steps));
+  p.scan = a;
+  return p;
+}
+
+template <bool BACK>
+void launch_scan(const Scan& in, int32_t dtype, dp_workspace ws, hipStream_t s) {
+  if (in.batch * in.channels == 0) return;
+  Plan p = plan_of<BACK>(in, element_bytes(dtype));
+  Scan& a = p.scan;
+  a.sums = reinterpret_cast<float*>(ws->scratch_only(
+      a.splits > 1 ? size_t(a.splits) * 2 * size_t(a.batch * a.channels) * sizeof(float) : 0));
+  with_element(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (p.line > 0) launch_typed<T, BACK, 1, 1>(a, p.waves, s);
+    else if (p.line < 0) launch_typed<T, BACK, 1, -1>(a, p.waves, s);
+    else if (p.width == 1) launch_typed<T, BACK, 1, 0>(a, p.waves, s);
+    else if constexpr (sizeof(T) == 2) launch_typed<T, BACK, 2, 0>(a, p.waves, s);
+  });
 }
 
 Scan scan_of(const dp_recurrence& r) {
   Scan a{};
   a.batch = r.batch;
   a.time = r.time;
-  a.channels = int32_t(r.channels);
+  a.channels = r.channels;
   return a;
 }
 
@@ -104,7 +420,7 @@ void check_recurrence(const dp_recurrence* r, int arrays) {
 }
 
 void launch_recurrence(const dp_recurrence& r, const void* gate, const void* value,
-                       const float* initial, void* state, float* last, dp_workspace,
+                       const float* initial, void* state, float* last, dp_workspace ws,
                        hipStream_t s) {
   Scan a = scan_of(r);
   a.down = r.reverse != 0;
@@ -116,12 +432,12 @@ void launch_recurrence(const dp_recurrence& r, const void* gate, const void* val
   a.gate_at = strides(r, 0);
   a.x_at = strides(r, 1);
   a.out_at = strides(r, 2);
-  launch_scan<false>(a, r.dtype, s);
+  launch_scan<false>(a, r.dtype, ws, s);
 }
 
 void launch_recurrence_backward(const dp_recurrence& r, const void* gate, const void* state,
                                 const void* dstate, const float* initial, const float* dlast,
-                                void* dgate, void* dvalue, float* dinitial, dp_workspace,
+                                void* dgate, void* dvalue, float* dinitial, dp_workspace ws,
                                 hipStream_t s) {
   Scan a = scan_of(r);
   a.down = r.reverse == 0;
@@ -138,7 +454,7 @@ void launch_recurrence_backward(const dp_recurrence& r, const void* gate, const 
   a.x_at = strides(r, 2);
   a.dgate_at = strides(r, 3);
   a.out_at = strides(r, 4);
-  launch_scan<true>(a, r.dtype, s);
+  launch_scan<true>(a, r.dtype, ws, s);
 }
 
 }  // namespace dp
