@@ -1,5 +1,7 @@
 """The operators over decisions against their definitions in 64 bits: log-probabilities of
 actions, the clipped policy loss, the preference loss, gated linear recurrences."""
+import zlib
+
 import numpy as np
 import policy_reference as ref64
 import pytest
@@ -17,7 +19,7 @@ def _rng(*key):
     import torch
 
     g = torch.Generator(device="cuda")
-    g.manual_seed(hash(key) % (1 << 31))
+    g.manual_seed(zlib.crc32(repr(key).encode()))  # hash() of a text differs by process
     return g
 
 
@@ -203,8 +205,9 @@ def test_border_of_the_clip_as_in_64_bits(ws, device, k):
     up = adv.cpu().numpy() > 0
     gap = (rows.logp - old.cpu().double().numpy()) - np.where(up, np.log1p(0.2), np.log1p(-0.2))
     active = np.where(up, gap < 0, gap > 0)
-    assert 0.2 < active.mean() < 0.8 and np.abs(gap).min() > 1e-12
-    assert np.array_equal(out.grad.abs().sum(1).cpu().numpy() > 0, active)
+    clear = np.abs(gap) > 1e-12  # nearer, 64 bits do not tell either
+    assert 0.2 < active.mean() < 0.8 and clear.mean() > 0.99
+    assert np.array_equal((out.grad.abs().sum(1).cpu().numpy() > 0)[clear], active[clear])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
