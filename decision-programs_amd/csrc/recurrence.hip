@@ -25,7 +25,7 @@
 namespace dp {
 namespace {
 
-constexpr int kMostWaves = 16;
+constexpr int kMostWaves = 8;  // of a workgroup
 
 struct Strides {
   int64_t batch, time;
@@ -41,6 +41,7 @@ struct Scan {
   int64_t batch_lanes; // over the channels of a batch
   int64_t first, groups;  // of lanes, one a workgroup: the launch's
   int64_t split_steps;
+  bool streamed;  // stores leave the caches to what is read again
   const void *gate, *x, *state;
   const float *initial, *carry;  // of the recurrence; the scan's start (null: zero)
   void *out, *dgate;
@@ -63,6 +64,9 @@ __device__ __forceinline__ Track<T> track(const Scan& a, P* base, const Strides&
   if (a.down) p += (a.time - 1) * at.time;
   return {p, a.down ? -at.time : at.time};
 }
+
+// A word at an element's alignment.
+typedef uint32_t Word __attribute__((aligned(2)));
 
 // STEPS steps of one array in registers: WIDTH neighbouring columns a step, or, where steps
 // are neighbours (LINE: 1 up, -1 down), vectors of steps.
@@ -130,7 +134,16 @@ struct Steps {
       for (int s = 0; s < STEPS; ++s, p += t.step) load_one(s, p);
     }
   }
-  __device__ __forceinline__ void store_all(const Track<T>& t, int64_t k) const {
+  __device__ __forceinline__ void store_all(const Track<T>& t, int64_t k, bool streamed) const {
+    if constexpr (LINE == 0 && WIDTH * sizeof(T) == 4) {
+      if (streamed) {
+        T* p = t.p + k * t.step;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s, p += t.step)
+          __builtin_nontemporal_store(w[s], reinterpret_cast<Word*>(p));
+        return;
+      }
+    }
     if constexpr (LINE != 0) {
       T* p = LINE > 0 ? t.p + k : t.p - k - (STEPS - 1);
 #pragma unroll
@@ -143,7 +156,8 @@ struct Steps {
   }
 };
 
-// SUMS: joins each split's steps only.
+// SUMS: joins each split's steps only, from the last block to the first, so that what is still
+// cached is what the next launch begins with.
 template <class T, bool BACK, bool SUMS, int STEPS, int WIDTH, int LINE>
 __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
   using Kept = Steps<T, STEPS, WIDTH, LINE>;
@@ -169,7 +183,8 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
   const auto dgate = track<T>(a, a.dgate, a.dgate_at, batch, channel);
 
   const int64_t begin = int64_t(split) * a.split_steps, end = min(begin + a.split_steps, a.time);
-  float h[WIDTH], through[WIDTH], first[WIDTH];  // the state before the block; SUMS: A so far
+  float h[WIDTH], first[WIDTH];  // the state before the block
+  float through[WIDTH];          // SUMS: A of the blocks so far, and h their B
 #pragma unroll
   for (int c = 0; c < WIDTH; ++c) {
     h[c] = !SUMS && a.carry && live ? a.carry[end_at + c] : 0.0f;
@@ -177,6 +192,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
     through[c] = 1.0f;
   }
   if (!SUMS && live)
+#pragma unroll 4
     for (unsigned i = 0; i < split; ++i) {
       const float* at = a.sums + 2 * i * all + end_at;
 #pragma unroll
@@ -184,8 +200,10 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
     }
 
   const int64_t block = int64_t(waves) * depth * STEPS;
-  int turn = 0;
-  for (int64_t k0 = begin; k0 < end; k0 += block, turn ^= 1) {
+  const int64_t blocks = end > begin ? (end - begin + block - 1) / block : 0;
+  for (int64_t i = 0; i < blocks; ++i) {
+    const int turn = int(i & 1);
+    const int64_t k0 = begin + (SUMS ? blocks - 1 - i : i) * block;
     const int64_t k = k0 + int64_t(wave * depth + along) * STEPS;
     // Whole: no step of the lane is outside, nor is the state that a backward step looks at.
     const bool whole = live && k + STEPS <= end && (!BACK || k + STEPS < a.time);
@@ -240,18 +258,25 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
       B[c] = along ? B0 : 0.0f;
     }
     __syncthreads();
+    if (SUMS) {
+#pragma unroll
+      for (int c = 0; c < WIDTH; ++c)
+        for (int w = waves - 1; w >= 0; --w) {
+          h[c] = fmaf(through[c], joined[turn][w][1][across * WIDTH + c], h[c]);
+          through[c] *= joined[turn][w][0][across * WIDTH + c];
+        }
+      continue;
+    }
     float mine[WIDTH];
 #pragma unroll
     for (int c = 0; c < WIDTH; ++c) {
       for (int w = 0; w < waves; ++w) {
         if (w == wave) mine[c] = h[c];
-        const float Aw = joined[turn][w][0][across * WIDTH + c];
-        h[c] = fmaf(Aw, h[c], joined[turn][w][1][across * WIDTH + c]);
-        if (SUMS) through[c] *= Aw;
+        h[c] = fmaf(joined[turn][w][0][across * WIDTH + c], h[c],
+                    joined[turn][w][1][across * WIDTH + c]);
       }
       mine[c] = fmaf(A[c], mine[c], B[c]);
     }
-    if (SUMS) continue;
     Kept o, da;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
@@ -271,8 +296,8 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
       if (BACK) da.set(s, d);
     }
     if (whole) {
-      o.store_all(out, k);
-      if (BACK) da.store_all(dgate, k);
+      o.store_all(out, k, a.streamed);
+      if (BACK) da.store_all(dgate, k, a.streamed);
     } else {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
@@ -294,101 +319,192 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
   }
 }
 
-template <bool BACK>
-constexpr int kSteps = BACK ? 8 : 16;
+// ---------------------------------------------------------------------------
+// A few steps (none, one new token, a short episode): a lane takes 16 bytes of channels through
+// all of them
+// ---------------------------------------------------------------------------
+constexpr int64_t kShortTime = 8;
+constexpr int kShortThreads = 256;
 
-template <class T, bool BACK, int WIDTH, int LINE>
-void launch_typed(Scan a, unsigned waves, hipStream_t s) {
-  constexpr int steps = kSteps<BACK>;
+template <class T, int WIDTH>
+struct Channels {
+  T v[WIDTH];
+
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(v, p, sizeof(v)); }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, v, sizeof(v)); }
+};
+
+template <class T, bool BACK, int WIDTH>
+__global__ __launch_bounds__(kShortThreads) void short_kernel(Scan a) {
+  const int64_t index = a.first + int64_t(blockIdx.x) * kShortThreads + threadIdx.x;
+  if (index >= a.batch * a.batch_lanes) return;
+  const int64_t batch = index / a.batch_lanes;
+  const int64_t channel =
+      min((index - batch * a.batch_lanes) * WIDTH, a.channels - int64_t(WIDTH));
+  const int64_t end_at = batch * a.channels + channel;
+  const auto gate = track<const T>(a, a.gate, a.gate_at, batch, channel);
+  const auto x = track<const T>(a, a.x, a.x_at, batch, channel);
+  const auto state = track<const T>(a, a.state, a.state_at, batch, channel);
+  const auto out = track<T>(a, a.out, a.out_at, batch, channel);
+  const auto dgate = track<T>(a, a.dgate, a.dgate_at, batch, channel);
+  float h[WIDTH];
+#pragma unroll
+  for (int c = 0; c < WIDTH; ++c) h[c] = a.carry ? a.carry[end_at + c] : 0.0f;
+#pragma unroll 2
+  for (int64_t k = 0; k < a.time; ++k) {
+    Channels<T, WIDTH> g, v, before, o, d;
+    g.load(gate.p + k * gate.step);
+    v.load(x.p + k * x.step);
+    const bool last = k + 1 == a.time;
+    if (BACK && !last) before.load(state.p + (k + 1) * state.step);
+#pragma unroll
+    for (int c = 0; c < WIDTH; ++c) {
+      if (BACK) {
+        const float y = float(v.v[c]) + h[c];
+        const float hp = !last ? float(before.v[c]) : a.initial ? a.initial[end_at + c] : 0.0f;
+        o.v[c] = T(y);
+        d.v[c] = T(y * hp);
+        h[c] = float(g.v[c]) * y;
+      } else {
+        h[c] = fmaf(float(g.v[c]), h[c], float(v.v[c]));
+        o.v[c] = T(h[c]);
+      }
+    }
+    o.store(out.p + k * out.step);
+    if (BACK) d.store(dgate.p + k * dgate.step);
+  }
+  if (a.end)
+#pragma unroll
+    for (int c = 0; c < WIDTH; ++c) a.end[end_at + c] = h[c];
+}
+
+template <class T, bool BACK, int WIDTH>
+void launch_short_width(Scan a, hipStream_t s) {
+  a.batch_lanes = (a.channels + WIDTH - 1) / WIDTH;
+  // A launch has fewer than 2^32 threads.
+  const int64_t lanes = a.batch * a.batch_lanes, most = int64_t(1) << 31;
+  for (a.first = 0; a.first < lanes; a.first += most)
+    short_kernel<T, BACK, WIDTH>
+        <<<unsigned((std::min(lanes - a.first, most) + kShortThreads - 1) / kShortThreads),
+           kShortThreads, 0, s>>>(a);
+  DP_HIP(hipGetLastError());
+}
+
+template <class T, bool BACK>
+void launch_short(const Scan& a, hipStream_t s) {
+  constexpr int wide = 16 / int(sizeof(T));
+  if (a.channels >= wide) launch_short_width<T, BACK, wide>(a, s);
+  else launch_short_width<T, BACK, 1>(a, s);
+}
+
+// ---------------------------------------------------------------------------
+// Which kernel
+// ---------------------------------------------------------------------------
+// Steps a lane.  Along a line a lane's steps are a vector or two; where channels lie side by
+// side, 16, or 8 where 16 would take too many registers (16 bit, unpacked in pairs) or where a
+// step takes few lanes (NARROW), so that the lanes of a wave stay close together in memory.
+template <class T, bool BACK, int LINE, bool NARROW>
+constexpr int kSteps = LINE ? (BACK ? 16 / int(sizeof(T)) : 8)
+                            : NARROW || (BACK && sizeof(T) == 2) ? 8 : 16;
+
+int64_t cover(int64_t n, int64_t by) { return (n + by - 1) / by; }
+int64_t power_of_two(int64_t n) { return int64_t(std::bit_ceil(uint64_t(n))); }
+
+constexpr int64_t kWorkgroups = 256;  // that fill the chip
+constexpr int64_t kMostSplits = 256;
+
+// Lays the scan on the chip; returns the waves of a workgroup.
+unsigned plan(Scan& a, int64_t steps, bool line, bool narrow) {
+  const int64_t lanes = a.batch * a.batch_lanes, parts = cover(a.time, steps);
+  int64_t across, most_waves = kMostWaves;
+  if (line) {
+    across = 64 / power_of_two(std::min<int64_t>(parts, 64));
+  } else if (narrow) {
+    // The channels of about two sequences side by side; fewer lanes where groups are few.
+    across = std::min<int64_t>(2 * power_of_two(a.batch_lanes), 64);
+    while (across > 8 && cover(lanes, across) < kWorkgroups * 5 / 4) across /= 2;
+    most_waves = 4;
+  } else {
+    // 256 bytes a step; 128 where that leaves one launch enough groups and 256 would not.
+    // 8 x 4096 x 2048 bfloat16: 97 us by 128 bytes, 123 by 256; 64 x 1000 x 512 float32: 84
+    // and 73.
+    across = power_of_two(std::min<int64_t>(lanes, 64));
+    if (cover(lanes, 64) < kWorkgroups * 9 / 16 && cover(lanes, 32) >= kWorkgroups * 7 / 16)
+      across = std::min<int64_t>(across, 32);
+  }
+  a.lanes = int32_t(across);
+  a.groups = cover(lanes, across);
+  const int64_t depth = 64 / across;
+  const int64_t waves = std::min(power_of_two(cover(parts, depth)), most_waves);
+  const int64_t block = waves * depth * steps, blocks = cover(a.time, block);
+  int64_t splits = 1;
+  if (a.groups < kWorkgroups * 7 / 16)
+    splits = std::min({cover(kWorkgroups, a.groups), blocks, kMostSplits});
+  a.split_steps = cover(blocks, splits) * block;
+  a.splits = int32_t(cover(a.time, a.split_steps));
+  a.streamed = across == 64 && a.batch_lanes >= 64;
+  return unsigned(waves);
+}
+
+template <class T, bool BACK, int WIDTH, int LINE, bool NARROW>
+void launch_plan(Scan a, dp_workspace ws, hipStream_t s) {
+  constexpr int steps = kSteps<T, BACK, LINE, NARROW>;
+  const unsigned threads = 64 * plan(a, steps, LINE != 0, NARROW);
   if (a.splits > 1) {
+    a.sums = reinterpret_cast<float*>(ws->scratch_only(
+        size_t(a.splits) * 2 * size_t(a.batch * a.channels) * sizeof(float)));
     const unsigned n = unsigned(a.groups);
     scan_kernel<T, BACK, true, steps, WIDTH, LINE>
-        <<<n * unsigned(a.splits - 1), waves * 64, 0, s>>>(a);
+        <<<n * unsigned(a.splits - 1), threads, 0, s>>>(a);
     DP_HIP(hipGetLastError());
     scan_kernel<T, BACK, false, steps, WIDTH, LINE>
-        <<<n * unsigned(a.splits), waves * 64, 0, s>>>(a);
+        <<<n * unsigned(a.splits), threads, 0, s>>>(a);
   } else {
     // A launch has fewer than 2^32 threads.
-    const int64_t most = int64_t(1) << 21, groups = a.groups;
+    const int64_t most = int64_t(1) << 22, groups = a.groups;
     for (a.first = 0; a.first < groups; a.first += most) {
       a.groups = std::min(groups - a.first, most);
       scan_kernel<T, BACK, false, steps, WIDTH, LINE>
-          <<<unsigned(a.groups), waves * 64, 0, s>>>(a);
+          <<<unsigned(a.groups), threads, 0, s>>>(a);
     }
   }
   DP_HIP(hipGetLastError());
 }
 
-int64_t cover(int64_t n, int64_t by) { return (n + by - 1) / by; }
-
-// How the scan lies on the chip.
-struct Plan {
-  Scan scan;
-  unsigned waves;  // of a workgroup
-  int line, width;
-};
-
-constexpr int64_t kWorkgroups = 512;  // that fill the chip
-constexpr int64_t kMostSplits = 64;
-
-template <bool BACK>
-Plan plan_of(Scan a, int element) {
-  Plan p{};
+template <class T, bool BACK>
+void launch_typed(Scan a, dp_workspace ws, hipStream_t s) {
   const Strides* at[] = {&a.gate_at, &a.x_at, &a.out_at, &a.state_at, &a.dgate_at};
-  bool merge = true, line = a.channels == 1;
+  bool merge = true, line = a.channels == 1 && a.time > 1;
   for (int i = 0; i < (BACK ? 5 : 3); ++i) {
     merge = merge && (a.batch == 1 || at[i]->batch == a.channels);
-    line = line && (a.time <= 1 || at[i]->time == 1);
+    line = line && at[i]->time == 1;
   }
   line = line && (a.batch == 1 || !merge);
   if (merge) {  // sequences side by side are channels
     a.channels *= a.batch;
     a.batch = 1;
   }
-  p.line = !line ? 0 : a.down ? -1 : 1;
-  p.width = element == 2 && a.channels >= 2 ? 2 : 1;
-  a.batch_lanes = cover(a.channels, p.width);
-
-  const int64_t lanes = a.batch * a.batch_lanes;
-  const int64_t parts = cover(std::max<int64_t>(a.time, 1), kSteps<BACK>);
-  const int64_t needed = int64_t(std::bit_ceil(uint64_t(std::min<int64_t>(parts, 64))));
-  int64_t across;
+  if (a.time <= kShortTime) return launch_short<T, BACK>(a, s);
+  const bool pairs = !line && sizeof(T) == 2 && a.channels >= 2;
+  a.batch_lanes = pairs ? cover(a.channels, 2) : a.channels;
+  const bool narrow = !line && a.batch_lanes < 32;
   if (line) {
-    across = 64 / needed;
+    if (a.down) launch_plan<T, BACK, 1, -1, false>(a, ws, s);
+    else launch_plan<T, BACK, 1, 1, false>(a, ws, s);
+  } else if constexpr (sizeof(T) == 2) {
+    if (!pairs) launch_plan<T, BACK, 1, 0, true>(a, ws, s);
+    else if (narrow) launch_plan<T, BACK, 2, 0, true>(a, ws, s);
+    else launch_plan<T, BACK, 2, 0, false>(a, ws, s);
   } else {
-    across = int64_t(std::bit_ceil(uint64_t(std::min<int64_t>(lanes, 64))));
-    // Narrower groups while there are too few, down to 32 bytes a step.
-    while (across > 8 && cover(lanes, across) < kWorkgroups && needed > 64 / across) across /= 2;
+    if (narrow) launch_plan<T, BACK, 1, 0, true>(a, ws, s);
+    else launch_plan<T, BACK, 1, 0, false>(a, ws, s);
   }
-  a.lanes = int32_t(across);
-  a.groups = cover(lanes, across);
-  const int64_t depth = 64 / across;
-  p.waves = unsigned(std::min<uint64_t>(std::bit_ceil(uint64_t(cover(parts, depth))), kMostWaves));
-  const int64_t block = int64_t(p.waves) * depth * kSteps<BACK>;
-  const int64_t blocks = cover(std::max<int64_t>(a.time, 1), block);
-  int64_t splits = 1;
-  if (a.groups < kWorkgroups / 2)
-    splits = std::min({cover(kWorkgroups, a.groups), blocks, kMostSplits});
-  a.split_steps = cover(blocks, splits) * block;
-  a.splits = int32_t(cover(std::max<int64_t>(a.time, 1), a.split_steps));
-  p.scan = a;
-  return p;
 }
 
 template <bool BACK>
-void launch_scan(const Scan& in, int32_t dtype, dp_workspace ws, hipStream_t s) {
-  if (in.batch * in.channels == 0) return;
-  Plan p = plan_of<BACK>(in, element_bytes(dtype));
-  Scan& a = p.scan;
-  a.sums = reinterpret_cast<float*>(ws->scratch_only(
-      a.splits > 1 ? size_t(a.splits) * 2 * size_t(a.batch * a.channels) * sizeof(float) : 0));
-  with_element(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (p.line > 0) launch_typed<T, BACK, 1, 1>(a, p.waves, s);
-    else if (p.line < 0) launch_typed<T, BACK, 1, -1>(a, p.waves, s);
-    else if (p.width == 1) launch_typed<T, BACK, 1, 0>(a, p.waves, s);
-    else if constexpr (sizeof(T) == 2) launch_typed<T, BACK, 2, 0>(a, p.waves, s);
-  });
+void launch_scan(const Scan& a, int32_t dtype, dp_workspace ws, hipStream_t s) {
+  if (a.batch * a.channels == 0) return;
+  with_element(dtype, [&](auto t) { launch_typed<decltype(t), BACK>(a, ws, s); });
 }
 
 Scan scan_of(const dp_recurrence& r) {

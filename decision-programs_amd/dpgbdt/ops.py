@@ -15,6 +15,19 @@ import numpy as np
 from . import BinLayout, Decisions, DPError, PolicyParam, PreferenceParam, Recurrence
 from . import SplitRecord, TrainParam, check, load
 
+
+class _Torch:
+    """Stands for torch until it is first used: the package itself imports without it."""
+
+    def __getattr__(self, name):
+        import torch as module
+
+        globals()["torch"] = module
+        return getattr(module, name)
+
+
+torch = _Torch()
+
 SPLIT_DTYPE = np.dtype([("loss_chg", "<f8"), ("gl", "<i8"), ("hl", "<i8"), ("feature", "<i4"),
                         ("bin", "<i4"), ("default_left", "<i4"), ("valid", "<i4"),
                         ("expand", "<i4"), ("pad", "<i4")])
@@ -22,13 +35,12 @@ assert SPLIT_DTYPE.itemsize == ctypes.sizeof(SplitRecord)
 
 
 def _stream():
-    import torch
-
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    # torch.cuda.current_stream().cuda_stream without the objects on the way
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t):
-    return c_void_p(t.data_ptr()) if t is not None else c_void_p(0)
+    return t.data_ptr() if t is not None else None
 
 
 class Workspace:
@@ -99,8 +111,6 @@ def sketch_cuts(ws, values, max_bin):
 
 def bin_values(values, lay, cut_ptr, cut_values):
     """Device bins (tile-major uint8 tensor) of a device float32 matrix."""
-    import torch
-
     dev = values.device
     cp = torch.as_tensor(np.asarray(cut_ptr, dtype=np.int32), device=dev)
     cv = torch.as_tensor(np.asarray(cut_values, dtype=np.float32), device=dev)
@@ -111,8 +121,6 @@ def bin_values(values, lay, cut_ptr, cut_values):
 
 
 def objective_gradients(objective, margin, label, n_classes):
-    import torch
-
     n = label.shape[0]
     grad = torch.empty((n, n_classes), dtype=torch.float32, device=margin.device)
     hess = torch.empty_like(grad)
@@ -123,8 +131,6 @@ def objective_gradients(objective, margin, label, n_classes):
 
 def quantise(ws, grad, hess):
     """-> (exps [K,2] int32, gpair [K,n,2] int32, sums [K,2] int64) device tensors."""
-    import torch
-
     if grad.dim() == 1:
         grad, hess = grad.reshape(-1, 1), hess.reshape(-1, 1)
     n, k = grad.shape
@@ -139,8 +145,6 @@ def quantise(ws, grad, hess):
 
 def hist_build(ws, bins, lay, gpair, segments, bin_stride, ridx=None, out=None):
     """Histograms [len(segments), F, bin_stride, 2] int64 of row segments."""
-    import torch
-
     seg = np.asarray(segments, dtype=np.int64).reshape(-1, 2)
     begin = np.ascontiguousarray(seg[:, 0])
     end = np.ascontiguousarray(seg[:, 1])
@@ -176,8 +180,6 @@ def hist_tuning(lay, bin_stride):
 
 
 def hist_subtract(parent, built):
-    import torch
-
     out = torch.empty_like(parent)
     check(load().dp_hist_subtract(_ptr(parent), _ptr(built), _ptr(out), parent.numel(), _stream()))
     return out
@@ -189,8 +191,6 @@ def train_param(eta=0.3, lam=1.0, alpha=0.0, gamma=0.0, min_child_weight=1.0, ma
 
 def evaluate_splits(ws, hist, n_bins, node_sums, exp_g, exp_h, param):
     """Best split per node -> device tensor of split records (see splits_to_numpy)."""
-    import torch
-
     n_nodes, f, stride, _ = hist.shape
     out = torch.empty((n_nodes, ctypes.sizeof(SplitRecord)), dtype=torch.uint8, device=hist.device)
     check(load().dp_evaluate_splits(ws.handle, _ptr(hist), n_nodes, f, stride, _ptr(n_bins),
@@ -206,8 +206,6 @@ def splits_to_numpy(records):
 
 def partition(ws, bins, lay, ridx_in, segments, splits):
     """Stable partition -> (ridx_out tensor, left_count tensor)."""
-    import torch
-
     seg = np.asarray(segments, dtype=np.int64).reshape(-1, 2)
     begin = np.ascontiguousarray(seg[:, 0])
     end = np.ascontiguousarray(seg[:, 1])
@@ -234,8 +232,6 @@ SYNTH_FEATURES = {1: 8, 2: 28, 3: 128, 4: 784, 5: 1000}
 
 def synth(config, n_rows, seed, device="cuda", n_features=None, want_grad=False):
     """Synthetic benchmark inputs -> (values, labels, grad, hess) device tensors."""
-    import torch
-
     f = n_features or SYNTH_FEATURES[config]
     values = torch.empty((n_rows, f), dtype=torch.float32, device=device)
     labels = torch.empty(n_rows, dtype=torch.float32, device=device)
@@ -255,49 +251,57 @@ PolicyLoss = collections.namedtuple("PolicyLoss", "loss logp kl entropy grad hes
 PreferenceLoss = collections.namedtuple("PreferenceLoss", "loss score logp grad hess")
 
 
-def _need(ok, message):
-    if not ok:
-        raise DPError(message)
-
-
 def _dtype(t, what):
-    import torch
-
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
-    _need(code is not None, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
-    return code
+    dtype = t.dtype
+    if dtype is torch.float32:
+        return 0
+    if dtype is torch.bfloat16:
+        return 2
+    if dtype is torch.float16:
+        return 1
+    raise DPError(f"{what} must be float32, float16 or bfloat16, not {dtype}")
 
 
 def _like(t, first, shape, what):
     """Checks a float32 array that goes with the tensor `first`."""
-    import torch
-
-    _need(t.dtype is torch.float32 and t.shape == shape and t.is_contiguous()
-          and t.device == first.device,
-          f"{what} must be a contiguous float32 tensor of shape {tuple(shape)} on {first.device}")
-    return t
+    if (t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous()
+            or t.device != first.device):
+        raise DPError(f"{what} must be a contiguous float32 tensor of shape {tuple(shape)} on "
+                      f"{first.device}")
 
 
 def _on_current_device(t, what):
-    import torch
-
-    _need(t.is_cuda and t.get_device() == torch.cuda.current_device(),
-          f"{what} must be on the current device")
+    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        raise DPError(f"{what} must be on the current device")
 
 
 def _decisions(margin, action):
-    import torch
-
-    _need(margin.dim() == 2, "margin must have shape [rows, classes]")
+    if margin.dim() != 2:
+        raise DPError("margin must have shape [rows, classes]")
     _on_current_device(margin, "margin")
     n, k = margin.shape
-    _need(k >= 1, "margin must have at least one class")
-    _need(margin.stride(1) == 1 or k == 1, "the classes of a row must be adjacent")
-    _need(action.dtype in (torch.int64, torch.int32) and action.shape == (n,)
-          and action.is_contiguous() and action.device == margin.device,
-          f"action must be a contiguous int64 or int32 tensor of shape ({n},) on {margin.device}")
-    return Decisions(margin.data_ptr(), action.data_ptr(), n, margin.stride(0), k,
-                     _dtype(margin, "margin"), action.element_size())
+    if k < 1:
+        raise DPError("margin must have at least one class")
+    row, step = margin.stride()
+    if step != 1 and k != 1:
+        raise DPError("the classes of a row must be adjacent")
+    wide = action.dtype is torch.int64
+    if (not (wide or action.dtype is torch.int32) or action.shape != (n,)
+            or not action.is_contiguous() or action.device != margin.device):
+        raise DPError(f"action must be a contiguous int64 or int32 tensor of shape ({n},) on "
+                      f"{margin.device}")
+    return Decisions(margin.data_ptr(), action.data_ptr(), n, row, k, _dtype(margin, "margin"),
+                     8 if wide else 4)
+
+
+def _floats(margin, *shape):
+    """An uninitialised float32 tensor beside margin."""
+    return torch.empty(shape, dtype=torch.float32, device=margin.device)
+
+
+def _gradient_of(margin):
+    """An uninitialised tensor for margin's gradient."""
+    return torch.empty_like(margin, memory_format=torch.contiguous_format)
 
 
 def action_logprobs(ws, margin, action, entropy=False):
@@ -306,24 +310,20 @@ def action_logprobs(ws, margin, action, entropy=False):
 
     Rows whose action is outside [0, K), or whose margins are all -infinity, are not counted: 0
     for both."""
-    import torch
-
     d = _decisions(margin, action)
-    logp = torch.empty(d.n_rows, dtype=torch.float32, device=margin.device)
-    h = torch.empty_like(logp) if entropy else None
+    logp = _floats(margin, d.n_rows)
+    h = _floats(margin, d.n_rows) if entropy else None
     check(load().dp_action_logprobs(ws.handle, ctypes.byref(d), _ptr(logp), _ptr(h), _stream()))
     return logp, h
 
 
 def action_logprobs_backward(ws, margin, action, dlogp, dentropy=None):
     """Gradient of the margins (their dtype, [n, K]) from those of action_logprobs' outputs."""
-    import torch
-
     d = _decisions(margin, action)
     _like(dlogp, margin, action.shape, "dlogp")
     if dentropy is not None:
         _like(dentropy, margin, action.shape, "dentropy")
-    grad = torch.empty(margin.shape, dtype=margin.dtype, device=margin.device)
+    grad = _gradient_of(margin)
     check(load().dp_action_logprobs_backward(ws.handle, ctypes.byref(d), _ptr(dlogp),
                                              _ptr(dentropy), _ptr(grad), _stream()))
     return grad
@@ -338,8 +338,6 @@ def policy_loss(ws, margin, action, old_logp, advantage, weight=None, reference=
     old_logp, advantage, weight and reference are float32 [n]; loss [n] holds the weighted rows,
     so its sum is what grad [n, K] is the gradient of.  hess (float32 margins only) is what
     Booster.boost takes beside grad.  kl is None without a reference, grad without gradient."""
-    import torch
-
     d = _decisions(margin, action)
     _like(old_logp, margin, action.shape, "old_logp")
     _like(advantage, margin, action.shape, "advantage")
@@ -347,14 +345,12 @@ def policy_loss(ws, margin, action, old_logp, advantage, weight=None, reference=
         _like(weight, margin, action.shape, "weight")
     if reference is not None:
         _like(reference, margin, action.shape, "reference")
-    _need(gradient or not hessian, "a hessian needs the gradient")
-    out = torch.empty((4, d.n_rows), dtype=torch.float32, device=margin.device)
-    loss, logp, k, h = out.unbind()
+    if hessian and not gradient:
+        raise DPError("a hessian needs the gradient")
+    loss, logp, k, h = _floats(margin, 4, d.n_rows).unbind()
     k = k if reference is not None else None
-    grad = (torch.empty(margin.shape, dtype=margin.dtype, device=margin.device)
-            if gradient else None)
-    hess = (torch.empty(margin.shape, dtype=torch.float32, device=margin.device)
-            if hessian else None)
+    grad = _gradient_of(margin) if gradient else None
+    hess = _floats(margin, d.n_rows, d.n_classes) if hessian else None
     param = PolicyParam(clip_low, clip_high, kl, entropy)
     check(load().dp_policy_loss(ws.handle, ctypes.byref(d), _ptr(old_logp), _ptr(advantage),
                                 _ptr(weight), _ptr(reference), ctypes.byref(param), _ptr(loss),
@@ -370,22 +366,21 @@ def preference_loss(ws, margin, action, sequences, reference=None, beta=0.1, smo
     sequences (int64 [2 P + 1], on the device) holds the offsets of the sequences' rows; pair i
     prefers sequence 2 i to sequence 2 i + 1.  reference (float32 [n]) holds the reference
     policy's log-probabilities of the actions; loss.sum() is what grad is the gradient of."""
-    import torch
-
     d = _decisions(margin, action)
-    _need(sequences.dtype is torch.int64 and sequences.dim() == 1 and sequences.is_contiguous()
-          and len(sequences) % 2 == 1 and sequences.device == margin.device,
-          f"sequences must be a contiguous int64 tensor of 2 P + 1 offsets on {margin.device}")
+    if (sequences.dtype is not torch.int64 or sequences.dim() != 1
+            or not sequences.is_contiguous() or len(sequences) % 2 != 1
+            or sequences.device != margin.device):
+        raise DPError(
+            f"sequences must be a contiguous int64 tensor of 2 P + 1 offsets on {margin.device}")
     if reference is not None:
         _like(reference, margin, action.shape, "reference")
-    _need(gradient or not hessian, "a hessian needs the gradient")
+    if hessian and not gradient:
+        raise DPError("a hessian needs the gradient")
     pairs = len(sequences) // 2
-    dev = margin.device
-    loss = torch.empty(pairs, dtype=torch.float32, device=dev)
-    score = torch.empty_like(loss)
-    logp = torch.empty(d.n_rows, dtype=torch.float32, device=dev)
-    grad = torch.empty(margin.shape, dtype=margin.dtype, device=dev) if gradient else None
-    hess = torch.empty(margin.shape, dtype=torch.float32, device=dev) if hessian else None
+    loss, score = _floats(margin, 2, pairs).unbind()
+    logp = _floats(margin, d.n_rows)
+    grad = _gradient_of(margin) if gradient else None
+    hess = _floats(margin, d.n_rows, d.n_classes) if hessian else None
     param = PreferenceParam(beta, smoothing, bool(average))
     check(load().dp_preference_loss(ws.handle, ctypes.byref(d), _ptr(sequences), pairs,
                                     _ptr(reference), ctypes.byref(param), _ptr(loss), _ptr(score),
@@ -395,30 +390,29 @@ def preference_loss(ws, margin, action, sequences, reference=None, beta=0.1, smo
 
 def _recurrence(reverse, arrays, ends):
     """The C description of [B, T, C] arrays and checks of the float32 [B, C] ones."""
-    import torch
-
-    first = arrays[0][0]
-    _need(first.dim() == 3, f"{arrays[0][1]} must have shape [batch, time, channels]")
-    _on_current_device(first, arrays[0][1])
-    b, t, c = first.shape
-    shape = Recurrence(b, t, c, _dtype(first, arrays[0][1]), bool(reverse))
-    for i, (x, what) in enumerate(arrays):
-        _need(x.dtype is first.dtype and x.shape == first.shape and x.device == first.device,
-              f"{what} must be {first.dtype} of shape {(b, t, c)} on {first.device}")
-        _need(c <= 1 or x.stride(2) == 1, f"the channels of {what} must be adjacent")
-        shape.strides[i][0], shape.strides[i][1] = x.stride(0), x.stride(1)
+    first, what = arrays[0]
+    if first.dim() != 3:
+        raise DPError(f"{what} must have shape [batch, time, channels]")
+    _on_current_device(first, what)
+    size, dtype, device = first.shape, first.dtype, first.device
+    b, t, c = size
+    shape = Recurrence(b, t, c, _dtype(first, what), bool(reverse))
+    for at, (x, what) in zip(shape.strides, arrays):
+        if x.dtype is not dtype or x.shape != size or x.device != device:
+            raise DPError(f"{what} must be {dtype} of shape {(b, t, c)} on {device}")
+        at[0], at[1], step = x.stride()
+        if step != 1 and c > 1:
+            raise DPError(f"the channels of {what} must be adjacent")
     for x, what in ends:
         if x is not None:
-            _like(x, first, torch.Size((b, c)), what)
+            _like(x, first, (b, c), what)
     return shape
 
 
 def _dense_like(x):
     """An empty tensor in x's order of dimensions, without its gaps or repeats."""
-    import torch
-
     out = torch.empty_like(x)  # keeps the strides of dense tensors only
-    return out if out.dim() != 3 or out.shape[2] <= 1 or out.stride(2) == 1 else out.contiguous()
+    return out if out.stride(2) == 1 or out.shape[2] <= 1 else out.contiguous()
 
 
 def linear_recurrence(ws, gate, value, initial=None, reverse=False):
@@ -430,12 +424,11 @@ def linear_recurrence(ws, gate, value, initial=None, reverse=False):
     channels are adjacent.  With a single step (T = 1) and initial = last of the call before, it
     is one step of a running recurrence.  Advantages: value the temporal differences, gate
     gamma * lambda, 0 where an episode ends, reverse=True."""
-    import torch
-
     shape = _recurrence(reverse, [(gate, "gate"), (value, "value")], [(initial, "initial")])
     state = _dense_like(value)
-    shape.strides[2][0], shape.strides[2][1] = state.stride(0), state.stride(1)
-    last = torch.empty((shape.batch, shape.channels), dtype=torch.float32, device=gate.device)
+    at = shape.strides[2]
+    at[0], at[1], _ = state.stride()
+    last = _floats(gate, shape.batch, shape.channels)
     check(load().dp_linear_recurrence(ws.handle, ctypes.byref(shape), _ptr(gate), _ptr(value),
                                       _ptr(initial), _ptr(state), _ptr(last), _stream()))
     return state, last
@@ -446,16 +439,14 @@ def linear_recurrence_backward(ws, gate, state, dstate, initial=None, dlast=None
     zero without) and the states it returned -> (dgate, dvalue, dinitial [B, C] float32).
 
     An input that was expanded has the sum of its gradient over the expanded dimension."""
-    import torch
-
     shape = _recurrence(reverse, [(gate, "gate"), (state, "state"), (dstate, "dstate")],
                         [(initial, "initial"), (dlast, "dlast")])
     dvalue = _dense_like(dstate)
-    dgate = torch.empty_strided(dvalue.shape, dvalue.stride(), dtype=gate.dtype,
-                                device=gate.device)
+    dgate = _dense_like(dvalue)
     for i, x in ((3, dgate), (4, dvalue)):
-        shape.strides[i][0], shape.strides[i][1] = x.stride(0), x.stride(1)
-    dinitial = torch.empty((shape.batch, shape.channels), dtype=torch.float32, device=gate.device)
+        at = shape.strides[i]
+        at[0], at[1], _ = x.stride()
+    dinitial = _floats(gate, shape.batch, shape.channels)
     check(load().dp_linear_recurrence_backward(ws.handle, ctypes.byref(shape), _ptr(gate),
                                                _ptr(state), _ptr(dstate), _ptr(initial),
                                                _ptr(dlast), _ptr(dgate), _ptr(dvalue),
