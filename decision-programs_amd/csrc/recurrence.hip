@@ -412,9 +412,12 @@ int64_t power_of_two(int64_t n) { return int64_t(std::bit_ceil(uint64_t(n))); }
 
 constexpr int64_t kWorkgroups = 256;  // that fill the chip
 constexpr int64_t kMostSplits = 256;
+// Results of this size leave the caches to what is read twice (4 x 32768 x 512 float32 backward
+// in two launches: 362 -> 338 us); smaller ones stay, for what takes them next.
+constexpr int64_t kStreamedBytes = int64_t(64) << 20;
 
 // Lays the scan on the chip; returns the waves of a workgroup.
-unsigned plan(Scan& a, int64_t steps, bool line, bool narrow) {
+unsigned plan(Scan& a, int64_t steps, int64_t element, bool line, bool narrow) {
   const int64_t lanes = a.batch * a.batch_lanes, parts = cover(a.time, steps);
   int64_t across, most_waves = kMostWaves;
   if (line) {
@@ -442,14 +445,15 @@ unsigned plan(Scan& a, int64_t steps, bool line, bool narrow) {
     splits = std::min({cover(kWorkgroups, a.groups), blocks, kMostSplits});
   a.split_steps = cover(blocks, splits) * block;
   a.splits = int32_t(cover(a.time, a.split_steps));
-  a.streamed = across == 64 && a.batch_lanes >= 64;
+  a.streamed = across == 64 && a.batch_lanes >= 64 &&
+               a.batch * a.channels * a.time * element >= kStreamedBytes;
   return unsigned(waves);
 }
 
 template <class T, bool BACK, int WIDTH, int LINE, bool NARROW>
 void launch_plan(Scan a, dp_workspace ws, hipStream_t s) {
   constexpr int steps = kSteps<T, BACK, LINE, NARROW>;
-  const unsigned threads = 64 * plan(a, steps, LINE != 0, NARROW);
+  const unsigned threads = 64 * plan(a, steps, sizeof(T), LINE != 0, NARROW);
   if (a.splits > 1) {
     a.sums = reinterpret_cast<float*>(ws->scratch_only(
         size_t(a.splits) * 2 * size_t(a.batch * a.channels) * sizeof(float)));
