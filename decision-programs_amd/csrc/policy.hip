@@ -616,7 +616,7 @@ __global__ __launch_bounds__(kThreads) void short_row_kernel(Rows a, uint32_t ma
 // The last vector of a row is one of the lanes' last ones: there are more than (NV - 1) LANES
 // and at most NV LANES.  It ends with the row, so that it holds elements of the one before again.
 template <int LANES, int NV>
-constexpr int kBatches = 16 / NV < LANES ? 16 / NV : LANES;
+constexpr int kBatches = NV == 1 ? (LANES < 16 ? LANES : 16) : NV == 2 ? 8 : 12 / NV;
 
 template <class T, int OP, bool HESS, int LANES, int NV>
 __global__ __launch_bounds__(kThreads, 4) void group_kernel(Rows a) {

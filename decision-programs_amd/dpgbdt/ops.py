@@ -265,7 +265,7 @@ def _dtype(t, what):
 def _like(t, first, shape, what):
     """Checks a float32 array that goes with the tensor `first`."""
     if (t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous()
-            or t.device != first.device):
+            or t.get_device() != first.get_device()):
         raise DPError(f"{what} must be a contiguous float32 tensor of shape {tuple(shape)} on "
                       f"{first.device}")
 
@@ -287,7 +287,7 @@ def _decisions(margin, action):
         raise DPError("the classes of a row must be adjacent")
     wide = action.dtype is torch.int64
     if (not (wide or action.dtype is torch.int32) or action.shape != (n,)
-            or not action.is_contiguous() or action.device != margin.device):
+            or not action.is_contiguous() or action.get_device() != margin.get_device()):
         raise DPError(f"action must be a contiguous int64 or int32 tensor of shape ({n},) on "
                       f"{margin.device}")
     return Decisions(margin.data_ptr(), action.data_ptr(), n, row, k, _dtype(margin, "margin"),
@@ -300,7 +300,7 @@ def _floats(margin, *shape):
 
 
 def _gradient_of(margin):
-    """An uninitialised tensor for margin's gradient."""
+    """An uninitialised tensor for margin's gradient or hessian."""
     return torch.empty_like(margin, memory_format=torch.contiguous_format)
 
 
@@ -350,7 +350,7 @@ def policy_loss(ws, margin, action, old_logp, advantage, weight=None, reference=
     loss, logp, k, h = _floats(margin, 4, d.n_rows).unbind()
     k = k if reference is not None else None
     grad = _gradient_of(margin) if gradient else None
-    hess = _floats(margin, d.n_rows, d.n_classes) if hessian else None
+    hess = _gradient_of(margin) if hessian else None
     param = PolicyParam(clip_low, clip_high, kl, entropy)
     check(load().dp_policy_loss(ws.handle, ctypes.byref(d), _ptr(old_logp), _ptr(advantage),
                                 _ptr(weight), _ptr(reference), ctypes.byref(param), _ptr(loss),
@@ -380,7 +380,7 @@ def preference_loss(ws, margin, action, sequences, reference=None, beta=0.1, smo
     loss, score = _floats(margin, 2, pairs).unbind()
     logp = _floats(margin, d.n_rows)
     grad = _gradient_of(margin) if gradient else None
-    hess = _floats(margin, d.n_rows, d.n_classes) if hessian else None
+    hess = _gradient_of(margin) if hessian else None
     param = PreferenceParam(beta, smoothing, bool(average))
     check(load().dp_preference_loss(ws.handle, ctypes.byref(d), _ptr(sequences), pairs,
                                     _ptr(reference), ctypes.byref(param), _ptr(loss), _ptr(score),
@@ -394,12 +394,12 @@ def _recurrence(reverse, arrays, ends):
     if first.dim() != 3:
         raise DPError(f"{what} must have shape [batch, time, channels]")
     _on_current_device(first, what)
-    size, dtype, device = first.shape, first.dtype, first.device
+    size, dtype, device = first.shape, first.dtype, first.get_device()
     b, t, c = size
     shape = Recurrence(b, t, c, _dtype(first, what), bool(reverse))
     for at, (x, what) in zip(shape.strides, arrays):
-        if x.dtype is not dtype or x.shape != size or x.device != device:
-            raise DPError(f"{what} must be {dtype} of shape {(b, t, c)} on {device}")
+        if x.dtype is not dtype or x.shape != size or x.get_device() != device:
+            raise DPError(f"{what} must be {dtype} of shape {(b, t, c)} on {first.device}")
         at[0], at[1], step = x.stride()
         if step != 1 and c > 1:
             raise DPError(f"the channels of {what} must be adjacent")
