@@ -277,6 +277,95 @@ def test_policy_gradient_is_the_slope_of_the_loss(ws, device):
         assert np.abs(slope - got[:, k])[clear].max() < 1e-6 * (1 + np.abs(got).max()) * 3
 
 
+# rows of each number of vectors a lane, whole and odd, on both sides of every change of kernel
+GROUPS = [17, 24, 32, 33, 48, 63, 66, 95, 127, 129, 191, 193, 255, 256, 258, 300, 384, 385, 511,
+          513, 700, 769, 800, 1023, 1024, 1025, 1500, 2047, 2048, 2049]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", GROUPS)
+def test_rows_of_a_wave(ws, device, k, dtype):
+    import torch
+    from dpgbdt import ops
+
+    z, y, old, adv, weight, reference = _case(k, dtype, n=301 if k < 300 else 75, illegal=0.1)
+    y[::5] = k - 1  # the end of a row, which may be held twice
+    weight[7], y[8] = 0.0, -1
+    z[7] = z[8] = float("nan")
+    z[9] = -float("inf")
+    old = torch.log_softmax(z.double(), 1).gather(1, y.clamp(min=0)[:, None])[:, 0]
+    old = (old.nan_to_num(0.0, 0.0, -20.0) - 0.05).float()
+    out = ops.policy_loss(ws, z, y, old, adv, weight, reference, kl=0.05, entropy=0.01,
+                          hessian=dtype == "float32")
+    some = [i for i in range(len(z)) if z[i, y[i]] != -float("inf")]
+    assert not any(x[7:10].any() for x in out if x is not None)
+    pick = type(out)(*(x if x is None else x[some] for x in out))
+    _check_policy(pick, z[some], y[some], old[some], adv[some], weight[some], reference[some],
+                  kl=0.05, entropy=0.01)
+    logp, h = ops.action_logprobs(ws, z, y, entropy=True)
+    counted = (weight != 0)
+    assert torch.equal(logp[counted], out.logp[counted])
+    assert torch.equal(h[counted], out.entropy[counted])
+
+
+@pytest.mark.parametrize("k", [2, 10, 32, 40, 300, 1000, 5000, 20000, 40000])
+def test_log_probabilities_next_to_zero(ws, device, k):
+    """A class that has almost everything: what is beside it decides, to its own precision."""
+    import torch
+    from dpgbdt import ops
+
+    g = _rng(k, "near")
+    z = torch.randn((40, k), generator=g, device="cuda") - 14.0 - float(np.log(k))
+    y = torch.randint(k, (40,), generator=g, device="cuda")
+    z.scatter_(1, y[:, None], 0.0)
+    logp, _ = ops.action_logprobs(ws, z, y)
+    want = torch.log_softmax(z.double(), 1).gather(1, y[:, None])[:, 0]
+    assert want.max() < 0 and want.min() > -1e-4
+    # exponentials are off by (|x| + 3) 2^-24 with |x| of up to 40 in powers of two, the sum's
+    # logarithm and its rounding by 2^-23
+    assert ((logp.double() - want).abs() <= want.abs() * (45 * 2.0 ** -24 + 2.0 ** -22)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [3, 10, 31, 33, 63, 130, 300, 513, 1030, 2050, 9001, 33001, 70001])
+def test_nothing_outside_the_rows(dp, ws, device, k, dtype):
+    """Margins between NaN and outputs between marks: neither is read nor written."""
+    import ctypes
+
+    import torch
+
+    n, edge = 13, 64
+    z, y, old, adv, weight, reference = _case(k, dtype, n=n)
+
+    def between(*shape, dtype=torch.float32, mark=float("nan")):
+        count = int(np.prod(shape))
+        whole = torch.full((count + 2 * edge,), mark, dtype=dtype, device="cuda")
+        return whole, whole[edge + 1:edge + 1 + count].view(shape)
+
+    held, zz = between(n, k, dtype=z.dtype)
+    zz.copy_(z)
+    code = {"float32": 0, "float16": 1, "bfloat16": 2}[dtype]
+    d = dp.Decisions(zz.data_ptr(), y.data_ptr(), n, k, k, code, 8)
+    param = dp.PolicyParam(0.2, 0.2, 0.05, 0.01)
+    outs = [between(n, mark=7.0) for _ in range(4)] + [between(n, k, dtype=z.dtype, mark=7.0)]
+    hess = between(n, k, mark=7.0)
+    ptr = [o[1].data_ptr() for o in outs]
+    dp.check(dp.load().dp_policy_loss(
+        ws.handle, ctypes.byref(d), old.data_ptr(), adv.data_ptr(), weight.data_ptr(),
+        reference.data_ptr(), ctypes.byref(param), *ptr,
+        hess[1].data_ptr() if dtype == "float32" else None,
+        torch.cuda.current_stream().cuda_stream))
+    for whole, inner in outs + [hess]:
+        count = inner.numel()
+        assert (whole[:edge + 1] == 7.0).all() and (whole[edge + 1 + count:] == 7.0).all()
+    from dpgbdt import ops
+
+    want = ops.policy_loss(ws, z, y, old, adv, weight, reference, kl=0.05, entropy=0.01,
+                           hessian=dtype == "float32")
+    got = [o[1] for o in outs] + ([hess[1]] if dtype == "float32" else [])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------------------
 # Preference loss
 # ---------------------------------------------------------------------------
@@ -514,6 +603,64 @@ def test_what_is_not_finite_stays_in_its_sequence(ws, device, b, t, c):
         assert torch.equal(state[1, :, 1:], clean[1, :, 1:])
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(5, 8, 13), (4, 3, 70), (7, 5, 9), (6, 2, 4), (3, 9, 5),
+                                   (2, 127, 64), (1, 128, 64), (2, 129, 97), (40, 130, 3),
+                                   (300, 140, 20), (20, 150, 31), (2, 385, 256), (1, 20000, 64),
+                                   (9, 4099, 1), (130, 33, 1), (130, 9, 1), (1, 16385, 1)])
+def test_recurrence_layouts(ws, device, shape, dtype, reverse):
+    """Every layout of lanes over steps and channels, its last block whole and not, and splits."""
+    gate, value, initial, dlast = _scan_case(shape, dtype)
+    _check_recurrence(ws, gate, value, initial, dlast, reverse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,t,c", [(2, 700, 67), (3, 5, 11), (1, 5000, 1), (70, 40, 3),
+                                   (1, 9000, 96)])
+def test_recurrence_writes_nothing_outside(dp, ws, device, b, t, c, dtype):
+    import ctypes
+
+    import torch
+
+    gate, value, initial, dlast = _scan_case((b, t, c), dtype)
+    edge, count = 64, b * t * c
+
+    def between(x=None, mark=float("nan")):
+        whole = torch.full((count + 2 * edge,), mark, dtype=gate.dtype, device="cuda")
+        inner = whole[edge + 1:edge + 1 + count].view(b, t, c)
+        if x is not None:
+            inner.copy_(x)
+        return whole, inner
+
+    from dpgbdt import ops
+
+    code = {"float32": 0, "float16": 1, "bfloat16": 2}[dtype]
+    for reverse in (False, True):
+        shape = dp.Recurrence(b, t, c, code, reverse)
+        for i in range(5):
+            shape.strides[i][0], shape.strides[i][1] = t * c, c
+        (_, g), (_, v) = between(gate), between(value)
+        out, da, dv = (between(mark=7.0) for _ in range(3))
+        stream = torch.cuda.current_stream().cuda_stream
+        last, dinitial = torch.empty((2, b, c), device="cuda").unbind()
+        dp.check(dp.load().dp_linear_recurrence(
+            ws.handle, ctypes.byref(shape), g.data_ptr(), v.data_ptr(), initial.data_ptr(),
+            out[1].data_ptr(), last.data_ptr(), stream))
+        state, end = ops.linear_recurrence(ws, gate, value, initial, reverse=reverse)
+        (_, s) = between(state)
+        dp.check(dp.load().dp_linear_recurrence_backward(
+            ws.handle, ctypes.byref(shape), g.data_ptr(), s.data_ptr(), v.data_ptr(),
+            initial.data_ptr(), dlast.data_ptr(), da[1].data_ptr(), dv[1].data_ptr(),
+            dinitial.data_ptr(), stream))
+        want = ops.linear_recurrence_backward(ws, gate, state, value, initial, dlast, reverse)
+        got = [out[1], last, da[1], dv[1], dinitial]
+        for x, w in zip(got, [state, end, *want]):
+            assert torch.equal(x, w)
+        for whole, _ in (out, da, dv):
+            assert (whole[:edge + 1] == 7.0).all() and (whole[edge + 1 + count:] == 7.0).all()
+
+
 # ---------------------------------------------------------------------------
 # Streams, graphs, far offsets
 # ---------------------------------------------------------------------------
@@ -583,6 +730,20 @@ def test_offsets_beyond_32_bits(ws, device):
         state, last = ops.linear_recurrence(ws, gate, view, initial)
         want, end = ops.linear_recurrence(ws, gate, value, initial)
         assert torch.equal(state, want) and torch.equal(last, end)
+
+
+def test_trees_learn_from_the_losses(dp, device):
+    """The example: the operators together with the booster they are for."""
+    import os
+    import sys
+
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(dp.__file__)), "..",
+                                    "examples"))
+    import train_policy
+
+    first, policy, preferences = train_policy.train(episodes=256, batches=8)
+    assert 0.2 < first < 0.3  # four actions
+    assert policy > 0.6 and preferences > policy - 0.02  # a sample of 2048 is off by 0.01
 
 
 # ---------------------------------------------------------------------------
