@@ -294,9 +294,11 @@ def _decisions(margin, action):
                      8 if wide else 4)
 
 
-def _floats(margin, *shape):
-    """An uninitialised float32 tensor beside margin."""
-    return torch.empty(shape, dtype=torch.float32, device=margin.device)
+def _floats(x, *shape):
+    """An uninitialised float32 tensor beside x."""
+    if x.dtype is torch.float32:
+        return x.new_empty(shape)
+    return torch.empty(shape, dtype=torch.float32, device=x.device)
 
 
 def _gradient_of(margin):
@@ -347,7 +349,7 @@ def policy_loss(ws, margin, action, old_logp, advantage, weight=None, reference=
         _like(reference, margin, action.shape, "reference")
     if hessian and not gradient:
         raise DPError("a hessian needs the gradient")
-    loss, logp, k, h = _floats(margin, 4, d.n_rows).unbind()
+    loss, logp, k, h = _floats(old_logp, 4, d.n_rows).unbind()
     k = k if reference is not None else None
     grad = _gradient_of(margin) if gradient else None
     hess = _gradient_of(margin) if hessian else None
