@@ -786,8 +786,9 @@ __global__ __launch_bounds__(WAVES * 64, row_waves(NV)) void row_kernel(Rows a) 
   const Span<T> span(k_all);
   const int full = int(span.full);
   // Vectors that start between words are read at 4/5 of the rate, so where nothing is stored a lane
-  // reads from the word that its vector starts in; the element behind is in what the lane after
-  // it read, or is read by itself.  3662 x 32767 bfloat16 scored in 54 us without, 49 with.
+  // reads from the word that its vector starts in (of the same allocation, then); the element
+  // behind is in what the lane after it read, or is read by itself.  3662 x 32767 bfloat16 scored
+  // in 54 us without, 49 with.
   const bool odd = OP == kScore && sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(row) & 2);
   Vec<T> v[NV];
   uint32_t behind[NV] = {};
@@ -949,7 +950,8 @@ __device__ __forceinline__ void finish_row(const Rows& a, int64_t r, RowIn& in, 
     if (fabs(gap) < kNearBorder) {
       double sum = 0.0;
 #pragma unroll 1
-      for (int k = tid; k < a.n_classes; k += THREADS) sum += exact_element(float(row[k]), st.m);
+      for (int64_t k = tid; k < a.n_classes; k += THREADS)
+        sum += exact_element(float(row[k]), st.m);
       gap = exact_gap(a, in, zy, st.m, block_sum<THREADS>(sum, part64));
       four.load(row + begin, span, tid);  // again: the 64-bit code has their registers meanwhile
     }
