@@ -614,10 +614,13 @@ __global__ __launch_bounds__(kThreads) void short_row_kernel(Rows a, uint32_t ma
 // A wave holds up to 64 rows in registers, kBatches batches of 64 / LANES rows of NV vectors a
 // lane.  Their statistics meet in LDS, where a lane takes a whole row: what a row costs by itself
 // (a logarithm, its loss, in 64 bits) is paid once for 64 rows, and read and written in order.
-// The last vector of a row is one of the lanes' last ones: there are more than (NV - 1) LANES
-// and at most NV LANES.  It ends with the row, so that it holds elements of the one before again.
+// The last vector of a row is one of the lanes' last kLast ones: there are more than
+// (NV - kLast) LANES and at most NV LANES.  It ends with the row, so that it holds elements of the
+// one before again.
 template <int LANES, int NV>
-constexpr int kBatches = NV == 1 ? (LANES < 16 ? LANES : 16) : NV == 2 ? 8 : 12 / NV;
+constexpr int kBatches = NV == 1 ? (LANES < 16 ? LANES : 16) : NV == 2 ? 8 : NV > 4 ? 1 : 12 / NV;
+template <int NV>
+constexpr int kLast = NV > 4 ? 2 : 1;
 
 template <class T, int OP, bool HESS, int LANES, int NV>
 __global__ __launch_bounds__(kThreads, 4) void group_kernel(Rows a) {
@@ -636,11 +639,11 @@ __global__ __launch_bounds__(kThreads, 4) void group_kernel(Rows a) {
   in.y = -1;
   if (live) in = row_in<OP>(a, r);
   const T* margin = static_cast<const T*>(a.margin);
-  const bool is_last = (NV - 1) * LANES + tid == vectors - 1;
-  // first element of vector j of this lane
-  const auto element = [&](int j) {
-    return j == NV - 1 && is_last ? k_all - N : (j * LANES + tid) * N;
+  const auto is_last = [&](int j) {
+    return j >= NV - kLast<NV> && j * LANES + tid == vectors - 1;
   };
+  // first element of vector j of this lane
+  const auto element = [&](int j) { return is_last(j) ? k_all - N : (j * LANES + tid) * N; };
   Vec<T> v[kAll][NV];
   const auto load = [&] {
 #pragma unroll
@@ -658,21 +661,27 @@ __global__ __launch_bounds__(kThreads, 4) void group_kernel(Rows a) {
   const float zy = in.y >= 0 ? float(margin[r * a.row_stride + in.y]) : 0.0f;
 #pragma unroll
   for (int b = 0; b < kAll; ++b) {
-    Vec<T> end = v[b][NV - 1];
-    if (again != 0)
+    // The last vector without what it holds again.
+    constexpr int kBefore = NV - kLast<NV>;
+    Vec<T> once[kLast<NV>];
 #pragma unroll
-      for (int e = 0; e < N - 1; ++e)
-        if (is_last && e < again) end.set(e, -INFINITY);
+    for (int i = 0; i < kLast<NV>; ++i) {
+      once[i] = v[b][kBefore + i];
+      if (again != 0)
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e)
+          if (is_last(kBefore + i) && e < again) once[i].set(e, -INFINITY);
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < N; ++e) top = fmaxf(top, (j == NV - 1 ? end : v[b][j]).get(e));
+      for (int e = 0; e < N; ++e)
+        top = fmaxf(top, (j < kBefore ? v[b][j] : once[j - kBefore]).get(e));
     Stats st{lanes_max<LANES>(top), 0.0f, 0.0};
     const float m = base_of(st.m);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      add_vec(j == NV - 1 ? end : v[b][j], m, st);
+    for (int j = 0; j < NV; ++j) add_vec(j < kBefore ? v[b][j] : once[j - kBefore], m, st);
 #pragma unroll
     for (int j = 0; j < NV; ++j) stay_packed(v[b][j]);
     st.s = lanes_sum<LANES>(st.s);
@@ -751,7 +760,7 @@ struct Span {
 // The row is read once, as NV vectors a thread and the single elements beside them, one a thread;
 // statistics and gradient come from the registers.
 // Waves a SIMD: as many as leave registers for the vectors and the row's 64-bit numbers.
-constexpr int row_waves(int nv) { return nv == 2 ? 7 : nv == 4 ? 6 : nv == 8 ? 5 : 4; }
+constexpr int row_waves(int nv) { return nv == 4 ? 6 : nv == 8 ? 5 : 4; }
 
 // Gradient (and hessian) of the elements of a row that is not counted.
 template <class T, bool HESS, int THREADS>
@@ -1088,7 +1097,7 @@ void launch_typed(Rows a, Pieces q, hipStream_t s) {
       else if (k <= 16) short_row_kernel<T, OP, HESS, 16><<<n, kThreads, lds, s>>>(a, magic);
       else short_row_kernel<T, OP, HESS, kShortRow><<<n, kThreads, lds, s>>>(a, magic);
     });
-  } else if (k <= 256 * Vec<T>::N) {
+  } else if (k <= 512 * Vec<T>::N) {
     const int64_t needed = (k + Vec<T>::N - 1) / Vec<T>::N;
     const auto group = [&]<int LANES, int NV>() {
       in_launches(a.n_rows, kThreads / LANES * kBatches<LANES, NV>,
@@ -1105,7 +1114,9 @@ void launch_typed(Rows a, Pieces q, hipStream_t s) {
     else if (needed <= 96) group.template operator()<32, 3>();
     else if (needed <= 128) group.template operator()<32, 4>();
     else if (needed <= 192) group.template operator()<64, 3>();
-    else group.template operator()<64, 4>();
+    else if (needed <= 256) group.template operator()<64, 4>();
+    else if (needed <= 384) group.template operator()<64, 6>();
+    else group.template operator()<64, 8>();
   } else if (q.count) {
     const unsigned n = unsigned(a.n_rows * q.count);
     piece_stats_kernel<T><<<n, kThreads, 0, s>>>(a, q, const_cast<Stats*>(q.stats));
@@ -1115,8 +1126,7 @@ void launch_typed(Rows a, Pieces q, hipStream_t s) {
   } else {
     in_launches(a.n_rows, 1, [&](int64_t first, unsigned n) {
       a.first = first;
-      if (vectors <= 512) row_kernel<T, OP, HESS, 2, 4><<<n, 256, 0, s>>>(a);
-      else if (vectors <= 1024) row_kernel<T, OP, HESS, 4, 4><<<n, 256, 0, s>>>(a);
+      if (vectors <= 1024) row_kernel<T, OP, HESS, 4, 4><<<n, 256, 0, s>>>(a);
       else if (vectors <= 2048) row_kernel<T, OP, HESS, 8, 4><<<n, 256, 0, s>>>(a);
       else if (vectors <= 4096) row_kernel<T, OP, HESS, 16, 4><<<n, 256, 0, s>>>(a);
       else if (vectors <= kRegisterVectors)

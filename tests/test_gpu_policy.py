@@ -279,7 +279,8 @@ def test_policy_gradient_is_the_slope_of_the_loss(ws, device):
 
 # rows of each number of vectors a lane, whole and odd, on both sides of every change of kernel
 GROUPS = [17, 24, 32, 33, 48, 63, 66, 95, 127, 129, 191, 193, 255, 256, 258, 300, 384, 385, 511,
-          513, 700, 769, 800, 1023, 1024, 1025, 1500, 2047, 2048, 2049]
+          513, 700, 769, 800, 1023, 1024, 1025, 1500, 2047, 2048, 2049, 2200, 2900, 3200, 3600,
+          4095, 4096, 4097]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
