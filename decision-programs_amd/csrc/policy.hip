@@ -11,9 +11,14 @@
 // A class whose margin is -infinity has probability zero and adds nothing; a row
 // without any other class is not counted.
 //
-// Statistics are held in 32 bits; log p_y, its differences to old and reference
-// log-probabilities and the sums over sequences in 64 bits: the difference of two
-// log-probabilities of about -10 that differ by 0.1 keeps 5 digits in 32.
+// Exponentials are 32-bit; their sums, log p_y, its differences to old and reference
+// log-probabilities and the sums over sequences are held in 64 bits: the difference
+// of two log-probabilities of about -10 that differ by 0.1 keeps 5 digits in 32.
+//
+// All kernels are bound by HBM where there is work for the whole chip, so each row is
+// read once if it can be held: in LDS and a thread's registers (short rows), in the
+// registers of some lanes, of a wave or of a workgroup.  Times below are of one MI355X,
+// where a large copy moves 4.8 TB/s.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -400,8 +405,8 @@ __device__ __forceinline__ void stay_packed(Vec<T>& o) {
     asm volatile("" : "+v"(o.w[0]), "+v"(o.w[1]), "+v"(o.w[2]), "+v"(o.w[3]));
 }
 
-// 16-bit margins, which are themselves off by 2^-9 of their size, are summed in 32 bits within a
-// vector.
+// 16-bit margins, which are themselves rounded by up to 2^-11 of their size or more, are summed in
+// 32 bits within a vector.
 template <class T>
 __device__ __forceinline__ void add_vec(const Vec<T>& v, float base, Stats& st) {
   if constexpr (sizeof(T) == 4) {
@@ -463,7 +468,9 @@ __device__ __forceinline__ void write_taken(float zy, const RowSlopes& g, T* gra
 // ---------------------------------------------------------------------------
 // A tile of 256 rows goes through LDS, so that memory is read and written in order whatever the
 // number of classes; a thread holds its row in registers.  Rows lie an odd number of words apart
-// there, which spreads the threads over the banks.
+// there, which spreads the threads over the banks.  A million rows of 10 classes with hessian: 36
+// us, 4.4 TB/s (a workgroup a row: 3,764); scoring 12 million 138 us, 4.8 TB/s.  From about 24
+// classes on the hessian's tile takes LDS from other workgroups: 32 run at 3.8 TB/s.
 constexpr int kShortRow = 32;
 constexpr int kTileRows = kThreads;
 
@@ -617,6 +624,8 @@ __global__ __launch_bounds__(kThreads) void short_row_kernel(Rows a, uint32_t ma
 // The last vector of a row is one of the lanes' last kLast ones: there are more than
 // (NV - kLast) LANES and at most NV LANES.  It ends with the row, so that it holds elements of the
 // one before again.
+// Scoring 1.9 million x 64 float32: 91 us, 5.6 TB/s (one batch a wave: 206); 80,000 x 1500: 79 us
+// (a workgroup a row: 125).  16-bit rows are bound by vector instructions, at 3 to 4.5 TB/s.
 template <int LANES, int NV>
 constexpr int kBatches = NV == 1 ? (LANES < 16 ? LANES : 16) : NV == 2 ? 8 : NV > 4 ? 1 : 12 / NV;
 template <int NV>
@@ -739,7 +748,7 @@ __global__ __launch_bounds__(kThreads, 4) void group_kernel(Rows a) {
 }
 
 // n elements of a row as whole vectors and the single ones behind them.  Which thread adds up
-// which elements does not go by where the row lies in memory: a row has the same bits in any batch.
+// which elements does not go by where the row lies in memory, and so do not its results.
 template <class T>
 struct Span {
   static constexpr int N = Vec<T>::N;
@@ -758,7 +767,10 @@ struct Span {
 // Rows of a workgroup
 // ---------------------------------------------------------------------------
 // The row is read once, as NV vectors a thread and the single elements beside them, one a thread;
-// statistics and gradient come from the registers.
+// statistics and gradient come from the registers.  8192 x 32768 bfloat16 policy loss: 209 us, 5.1
+// TB/s, the vector units 70 % busy; scoring 4096 x 50021 85 us, 84 % busy.  Workgroups of 256 to
+// 512 threads with many registers, of which 2 to 4 on a compute unit are in different phases, beat
+// one of 1024 (225 us).
 // Waves a SIMD: as many as leave registers for the vectors and the row's 64-bit numbers.
 constexpr int row_waves(int nv) { return nv == 4 ? 6 : nv == 8 ? 5 : 4; }
 
@@ -985,7 +997,8 @@ __device__ __forceinline__ void finish_row(const Rows& a, int64_t r, RowIn& in, 
   if (y >= 0 && y < span.size && tid == span.owner(y, THREADS)) write_taken(zy, g, grad, int(y));
 }
 
-// A workgroup a row, which it reads twice.
+// A workgroup a row, which it reads twice, the second time from the 256 MB behind the L2s for the
+// most part.  Policy loss of 2000 x 50021 float32: 177 us for the 800 MB read and written once.
 constexpr int kLongThreads = 1024;
 
 template <class T, int OP, bool HESS>
@@ -1007,7 +1020,8 @@ __global__ __launch_bounds__(kLongThreads, 8) void long_row_kernel(Rows a) {
 
 // A workgroup a piece of a row.  Few rows take two launches: statistics of the pieces, of rows that
 // are not counted too, then each piece's gradient from all of the row's statistics.  The second
-// serves any number of rows whose statistics are there already.
+// serves any number of rows whose statistics are there already.  24 x 131071 float32: 6 and 7 us,
+// of launch and dependent loads; 25 MB would take 5.
 struct Pieces {
   int64_t elements;  // of a piece: whole vectors
   int32_t count;     // of a row
@@ -1214,7 +1228,9 @@ __device__ __forceinline__ PairRows pair_rows(const Pairs& a, int64_t pair) {
   return {row(2 * pair), row(2 * pair + 1), row(2 * pair + 2)};
 }
 
-// A pair by `size` threads, of which this is thread tid; sum(v) adds over them.
+// A pair by `size` threads, of which this is thread tid; sum(v) adds over them.  Bound by latency:
+// offsets, log-probabilities, then an exponential and a logarithm in 64 bits, 6 to 7 us for 500
+// pairs of 60,000 rows or 16 of 16,384.
 template <class Sum>
 __device__ __forceinline__ void one_pair(const Pairs& a, int64_t pair, const PairRows& at, int tid,
                                          int size, Sum&& sum) {

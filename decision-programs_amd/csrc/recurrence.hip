@@ -7,6 +7,9 @@
 // passes are one scan, of h or of c: a step is h -> a h + b forward and
 // c -> a (dh + c) backward, and steps join as pairs (A, B): x -> A x + B.
 //
+// Bound by HBM: two or three arrays are read and one or two written, a few operations
+// an element.  Times below are of one MI355X, where a large copy moves 4.8 TB/s.
+//
 // A lane takes kSteps neighbouring steps of its columns into registers and joins
 // them; the lanes of a wave, then its workgroup's waves, join theirs; with the state
 // before them the steps are taken again, from the registers, and stored.  So the
@@ -14,6 +17,10 @@
 // these leave.  Where the columns do not fill the chip, time is split over
 // workgroups: one launch joins each split's steps, the next starts from the splits
 // before, and both gate and values are read twice.
+//   forward 8 x 4096 x 2048 bfloat16, one launch: 97 us, 4.2 TB/s
+//   backward 4 x 32768 x 512 float32, 32 groups of channels by 8 splits: 97 and 250 us
+//     (5.5 and 5.4 TB/s; by narrower groups in one launch 446)
+//   forward 300 x 200000 x 1 float32, along time: 164 us, 4.4 TB/s
 //
 // States are held in 32 bits and rounded once where they are stored in 16.
 #include <algorithm>
@@ -335,7 +342,11 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
 // A few steps (none, one new token, a short episode): a lane takes 16 bytes of channels through
 // all of them
 // ---------------------------------------------------------------------------
+// Forward, bfloat16, against the scan: 4096 x 1 x 1024 14 us (42), 2048 x 4 x 1024 12 (25),
+// 1024 x 16 x 1024 18.6 (19.9), 512 x 32 x 1024 18.7 (17.6).
 constexpr int64_t kShortTime = 8;
+constexpr int64_t kShortTimeOfMany = 16;  // where lanes fill the chip
+constexpr int64_t kManyLanes = 65536;
 constexpr int kShortThreads = 256;
 
 template <class T, int WIDTH>
@@ -362,7 +373,7 @@ __global__ __launch_bounds__(kShortThreads) void short_kernel(Scan a) {
   float h[WIDTH];
 #pragma unroll
   for (int c = 0; c < WIDTH; ++c) h[c] = a.carry ? a.carry[end_at + c] : 0.0f;
-#pragma unroll 2
+#pragma unroll 4
   for (int64_t k = 0; k < a.time; ++k) {
     Channels<T, WIDTH> g, v, before, o, d;
     g.load(gate.p + k * gate.step);
@@ -412,9 +423,11 @@ void launch_short(const Scan& a, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // Which kernel
 // ---------------------------------------------------------------------------
-// Steps a lane.  Along a line a lane's steps are a vector or two; where channels lie side by
-// side, 16, or 8 where 16 would take too many registers (16 bit, unpacked in pairs) or where a
-// step takes few lanes (NARROW), so that the lanes of a wave stay close together in memory.
+// Steps a lane.  Along a line a lane's steps are a vector or two (backward of 300 x 200000 x 1
+// float32: 262 us by one vector, 301 by two; forward 171 and 164).  Where channels lie side by
+// side, 16, or 8 where 16 would take too many registers (16 bit, unpacked in pairs: backward of
+// 512 x 256 x 256 68 us by 8, 80 by 16) or where a step takes few lanes (NARROW), so that the
+// lanes of a wave stay close together in memory (forward of 2000 x 1000 x 3: 24 and 38).
 template <class T, bool BACK, int LINE, bool NARROW>
 constexpr int kSteps = LINE ? (BACK ? 16 / int(sizeof(T)) : 8)
                             : NARROW || (BACK && sizeof(T) == 2) ? 8 : 16;
@@ -503,7 +516,9 @@ void launch_typed(Scan a, dp_workspace ws, hipStream_t s) {
     a.channels *= a.batch;
     a.batch = 1;
   }
-  if (a.time <= kShortTime) return launch_short<T, BACK>(a, s);
+  const int64_t vectors = a.batch * (a.channels * int64_t(sizeof(T)) / 16);
+  if (a.time <= (vectors >= kManyLanes ? kShortTimeOfMany : kShortTime))
+    return launch_short<T, BACK>(a, s);
   const bool pairs = !line && sizeof(T) == 2 && a.channels >= 2;
   a.batch_lanes = pairs ? cover(a.channels, 2) : a.channels;
   const bool narrow = !line && a.batch_lanes < 32;

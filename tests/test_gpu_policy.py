@@ -609,7 +609,8 @@ def test_what_is_not_finite_stays_in_its_sequence(ws, device, b, t, c):
 @pytest.mark.parametrize("shape", [(5, 8, 13), (4, 3, 70), (7, 5, 9), (6, 2, 4), (3, 9, 5),
                                    (2, 127, 64), (1, 128, 64), (2, 129, 97), (40, 130, 3),
                                    (300, 140, 20), (20, 150, 31), (2, 385, 256), (1, 20000, 64),
-                                   (9, 4099, 1), (130, 33, 1), (130, 9, 1), (1, 16385, 1)])
+                                   (9, 4099, 1), (130, 33, 1), (130, 9, 1), (1, 16385, 1),
+                                   (2100, 16, 130), (1100, 11, 256), (1, 16, 70)])
 def test_recurrence_layouts(ws, device, shape, dtype, reverse):
     """Every layout of lanes over steps and channels, its last block whole and not, and splits."""
     gate, value, initial, dlast = _scan_case(shape, dtype)
