@@ -376,13 +376,15 @@ int dp_update_margin(dp_workspace ws, const uint32_t* ridx, const int64_t* begin
  * With n_classes logits a row, p = softmax(margin) and y the action of the row:
  *   log p_y, entropy H = -sum p log p.
  * A row whose action is outside [0, n_classes) or whose weight is 0 is not
- * counted: its margins are not looked at (they may hold NaN), its outputs,
- * gradient and hessian are 0.  A class whose margin is -infinity has probability
- * 0 and gradient 0; a row with no other class is not counted either.  NaN in a counted row reaches that row's outputs only
- * (and its pair's).  Sums and statistics are held in 32 bits or more, log p_y
- * and its differences in 64; the same call gives the same bits every time.
- * The calls allocate nothing once the workspace has grown to their size, and
- * can be captured into a graph then. */
+ * counted: its margins may hold anything (NaN too), its outputs, gradient and
+ * hessian are 0.  A class whose margin is -infinity has probability 0 and
+ * gradient 0; a row with no other class is not counted either.  NaN in a counted
+ * row reaches that row's outputs only (and its pair's).  Sums of exponentials,
+ * log p_y and its differences are held in 64 bits (sums of 16-bit margins in 32
+ * over 8 classes); the same call gives the same bits every time, and log p_y of
+ * the same margins is the same in every call.  Any row stride will do.
+ * The calls allocate nothing once the workspace has grown to their size, and can
+ * be captured into a graph then.  Use one stream at a time per workspace. */
 enum dp_dtype { DP_FLOAT32 = 0, DP_FLOAT16 = 1, DP_BFLOAT16 = 2 };
 
 typedef struct {
