@@ -17,9 +17,9 @@
 // these leave.  Where the columns do not fill the chip, time is split over
 // workgroups: one launch joins each split's steps, the next starts from the splits
 // before, and both gate and values are read twice.
-//   forward 8 x 4096 x 2048 bfloat16, one launch: 97 us, 4.2 TB/s
-//   backward 4 x 32768 x 512 float32, 32 groups of channels by 8 splits: 97 and 250 us
-//     (5.5 and 5.4 TB/s; by narrower groups in one launch 446)
+//   forward 8 x 4096 x 2048 bfloat16, one launch: 92 us, 4.4 TB/s
+//   backward 4 x 32768 x 512 float32, 32 groups of channels by 8 splits: 96 and 243 us
+//     (5.5 TB/s; by narrower groups in one launch 446 together)
 //   forward 300 x 200000 x 1 float32, along time: 164 us, 4.4 TB/s
 //
 // States are held in 32 bits and rounded once where they are stored in 16.
@@ -173,8 +173,11 @@ struct Steps {
 };
 
 // SUMS: joins each split's steps only, from the last block to the first, so that what is still
-// cached is what the next launch begins with.
-template <class T, bool BACK, bool SUMS, int STEPS, int WIDTH, int LINE>
+// cached is what the next launch begins with.  AHEAD: a block's steps are read before the one
+// before it is joined, in registers that only a compute unit with one workgroup has to spare:
+// 8 x 4096 x 2048 bfloat16 forward 97 -> 92 us, backward 164 -> 146; 4 x 32768 x 512 bfloat16
+// backward, in two launches, 220 -> 198.
+template <class T, bool BACK, bool SUMS, int STEPS, int WIDTH, int LINE, bool AHEAD>
 __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
   using Kept = Steps<T, STEPS, WIDTH, LINE>;
   __shared__ float joined[2][kMostWaves][2][64 * WIDTH];
@@ -220,34 +223,55 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
 
   const int64_t block = int64_t(waves) * depth * STEPS;
   const int64_t blocks = end > begin ? (end - begin + block - 1) / block : 0;
-  for (int64_t i = 0; i < blocks; ++i) {
-    const int turn = int(i & 1);
-    const int64_t k0 = begin + (SUMS ? blocks - 1 - i : i) * block;
-    const int64_t k = k0 + int64_t(wave * depth + along) * STEPS;
-    // Whole: no step of the lane is outside, nor is the state that a backward step looks at.
-    const bool whole = live && k + STEPS <= end && (!BACK || k + STEPS < a.time);
-    const int count = !live ? 0 : int(min(max(end - k, int64_t(0)), int64_t(STEPS)));
+  struct Block {
     Kept g, v, before;
-    if (whole) {
-      g.load_all(gate, k);
-      v.load_all(x, k);
-      if (BACK && !SUMS) before.load_all(state, k + 1);
+  };
+  const auto step_of = [&](int64_t i) {
+    return begin + (SUMS ? blocks - 1 - i : i) * block + int64_t(wave * depth + along) * STEPS;
+  };
+  // Whole: no step of the lane is outside, nor is the state that a backward step looks at.
+  const auto is_whole = [&](int64_t k) {
+    return live && k + STEPS <= end && (!BACK || k + STEPS < a.time);
+  };
+  const auto count_of = [&](int64_t k) {
+    return !live ? 0 : int(min(max(end - k, int64_t(0)), int64_t(STEPS)));
+  };
+  const auto load = [&](int64_t k, Block& o) {
+    if (is_whole(k)) {
+      o.g.load_all(gate, k);
+      o.v.load_all(x, k);
+      if (BACK && !SUMS) o.before.load_all(state, k + 1);
     } else {
       // Steps outside keep the state.
       const float one[2] = {1.0f, 1.0f}, zero[2] = {0.0f, 0.0f};
+      const int count = count_of(k);
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        g.set(s, one);
-        v.set(s, zero);
-        if (BACK && !SUMS) before.set(s, zero);
+        o.g.set(s, one);
+        o.v.set(s, zero);
+        if (BACK && !SUMS) o.before.set(s, zero);
         if (s < count) {
-          g.load_one(s, gate.p + (k + s) * gate.step);
-          v.load_one(s, x.p + (k + s) * x.step);
+          o.g.load_one(s, gate.p + (k + s) * gate.step);
+          o.v.load_one(s, x.p + (k + s) * x.step);
           if (BACK && !SUMS && k + s + 1 < a.time)
-            before.load_one(s, state.p + (k + s + 1) * state.step);
+            o.before.load_one(s, state.p + (k + s + 1) * state.step);
         }
       }
     }
+  };
+  Block next;
+  if (AHEAD && blocks) load(step_of(0), next);
+  for (int64_t i = 0; i < blocks; ++i) {
+    const int turn = int(i & 1);
+    const int64_t k = step_of(i);
+    Block now;
+    if (AHEAD) {
+      now = next;
+      if (i + 1 < blocks) load(step_of(i + 1), next);
+    } else {
+      load(k, now);
+    }
+    const Kept &g = now.g, &v = now.v, &before = now.before;
     float A[WIDTH], B[WIDTH];
 #pragma unroll
     for (int c = 0; c < WIDTH; ++c) {
@@ -314,10 +338,11 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
       o.set(s, y);
       if (BACK) da.set(s, d);
     }
-    if (whole) {
+    if (is_whole(k)) {
       o.store_all(out, k, a.streamed);
       if (BACK) da.store_all(dgate, k, a.streamed);
     } else {
+      const int count = count_of(k);
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
         if (s < count) {
@@ -456,8 +481,8 @@ unsigned plan(Scan& a, int64_t steps, int64_t element, bool line, bool narrow) {
     most_waves = 4;
   } else {
     // 256 bytes a step; 128 where that leaves one launch enough groups and 256 would not.
-    // 8 x 4096 x 2048 bfloat16: 97 us by 128 bytes, 123 by 256; 64 x 1000 x 512 float32: 84
-    // and 73.
+    // 8 x 4096 x 2048 bfloat16: 97 us by 128 bytes, 123 by 256 (neither read ahead);
+    // 64 x 1000 x 512 float32: 84 and 73.
     across = power_of_two(std::min<int64_t>(lanes, 64));
     if (cover(lanes, 64) < kWorkgroups * 9 / 16 && cover(lanes, 32) >= kWorkgroups * 7 / 16)
       across = std::min<int64_t>(across, 32);
@@ -478,25 +503,30 @@ unsigned plan(Scan& a, int64_t steps, int64_t element, bool line, bool narrow) {
   return unsigned(waves);
 }
 
+// The splits, or so few groups, are about a workgroup for every compute unit: these read ahead.
 template <class T, bool BACK, int WIDTH, int LINE, bool NARROW>
 void launch_plan(Scan a, dp_workspace ws, hipStream_t s) {
   constexpr int steps = kSteps<T, BACK, LINE, NARROW>;
+  constexpr bool kAhead = !NARROW && !LINE;
   const unsigned threads = 64 * plan(a, steps, sizeof(T), LINE != 0, NARROW);
   if (a.splits > 1) {
     a.sums = reinterpret_cast<float*>(ws->scratch_only(
         size_t(a.splits) * 2 * size_t(a.batch * a.channels) * sizeof(float)));
     const unsigned n = unsigned(a.groups);
-    scan_kernel<T, BACK, true, steps, WIDTH, LINE>
+    scan_kernel<T, BACK, true, steps, WIDTH, LINE, false>
         <<<n * unsigned(a.splits - 1), threads, 0, s>>>(a);
     DP_HIP(hipGetLastError());
-    scan_kernel<T, BACK, false, steps, WIDTH, LINE>
+    scan_kernel<T, BACK, false, steps, WIDTH, LINE, kAhead>
         <<<n * unsigned(a.splits), threads, 0, s>>>(a);
+  } else if (kAhead && a.groups <= kWorkgroups) {
+    scan_kernel<T, BACK, false, steps, WIDTH, LINE, kAhead>
+        <<<unsigned(a.groups), threads, 0, s>>>(a);
   } else {
     // A launch has fewer than 2^32 threads.
     const int64_t most = int64_t(1) << 22, groups = a.groups;
     for (a.first = 0; a.first < groups; a.first += most) {
       a.groups = std::min(groups - a.first, most);
-      scan_kernel<T, BACK, false, steps, WIDTH, LINE>
+      scan_kernel<T, BACK, false, steps, WIDTH, LINE, false>
           <<<unsigned(a.groups), threads, 0, s>>>(a);
     }
   }

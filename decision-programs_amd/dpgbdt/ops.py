@@ -349,14 +349,19 @@ def policy_loss(ws, margin, action, old_logp, advantage, weight=None, reference=
         _like(reference, margin, action.shape, "reference")
     if hessian and not gradient:
         raise DPError("a hessian needs the gradient")
-    loss, logp, k, h = _floats(old_logp, 4, d.n_rows).unbind()
-    k = k if reference is not None else None
+    rows = _floats(old_logp, 4, d.n_rows)
+    at, step = rows.data_ptr(), 4 * d.n_rows
+    loss, logp, k, h = rows.unbind()
+    k_at = at + 2 * step
+    if reference is None:
+        k = k_at = None
     grad = _gradient_of(margin) if gradient else None
     hess = _gradient_of(margin) if hessian else None
     param = PolicyParam(clip_low, clip_high, kl, entropy)
-    check(load().dp_policy_loss(ws.handle, ctypes.byref(d), _ptr(old_logp), _ptr(advantage),
-                                _ptr(weight), _ptr(reference), ctypes.byref(param), _ptr(loss),
-                                _ptr(logp), _ptr(k), _ptr(h), _ptr(grad), _ptr(hess), _stream()))
+    check(load().dp_policy_loss(ws.handle, ctypes.byref(d), old_logp.data_ptr(),
+                                advantage.data_ptr(), _ptr(weight), _ptr(reference),
+                                ctypes.byref(param), at, at + step, k_at, at + 3 * step,
+                                _ptr(grad), _ptr(hess), _stream()))
     return PolicyLoss(loss, logp, k, h, grad, hess)
 
 
