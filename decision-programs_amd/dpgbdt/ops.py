@@ -51,9 +51,9 @@ class Workspace:
         check(load().dp_workspace_create(ctypes.byref(self.handle)))
 
     def __del__(self):
-        lib = load()
-        if getattr(self, "handle", None):
-            lib.dp_workspace_free(self.handle)
+        # load is None when the interpreter has taken the module down already
+        if getattr(self, "handle", None) and load is not None:
+            load().dp_workspace_free(self.handle)
             self.handle = None
 
 
