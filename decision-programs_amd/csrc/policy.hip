@@ -180,7 +180,8 @@ __device__ __forceinline__ V over_lanes(V v, Op&& op) {
       };
       const Words w = __builtin_bit_cast(Words, v);
       const Halves lo = halves<LANES>(w.w[0]), hi = halves<LANES>(w.w[1]);
-      return op(__builtin_bit_cast(V, Words{{lo.a, hi.a}}), __builtin_bit_cast(V, Words{{lo.b, hi.b}}));
+      return op(__builtin_bit_cast(V, Words{{lo.a, hi.a}}),
+                __builtin_bit_cast(V, Words{{lo.b, hi.b}}));
     }
   }
 }

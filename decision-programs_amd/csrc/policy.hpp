@@ -33,21 +33,6 @@ void launch_recurrence_backward(const dp_recurrence& r, const void* gate, const 
                                 hipStream_t s);
 
 // ---- element types ---------------------------------------------------------
-template <int DTYPE>
-struct Element;
-template <>
-struct Element<DP_FLOAT32> {
-  using type = float;
-};
-template <>
-struct Element<DP_FLOAT16> {
-  using type = _Float16;
-};
-template <>
-struct Element<DP_BFLOAT16> {
-  using type = __bf16;
-};
-
 inline int element_bytes(int32_t dtype) { return dtype == DP_FLOAT32 ? 4 : 2; }
 
 // Calls f(T{}) with the element type of `dtype` (checked before).
