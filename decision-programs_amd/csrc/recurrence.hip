@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void scan_kernel(Scan a) {
     through[c] = 1.0f;
   }
   if (!SUMS && live)
-#pragma unroll 4
+#pragma unroll 8
     for (unsigned i = 0; i < split; ++i) {
       const float* at = a.sums + 2 * i * all + end_at;
 #pragma unroll
