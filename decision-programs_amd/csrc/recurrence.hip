@@ -494,8 +494,11 @@ unsigned plan(Scan& a, int64_t steps, int64_t element, bool line, bool narrow) {
   const int64_t waves = std::min(power_of_two(cover(parts, depth)), most_waves);
   const int64_t block = waves * depth * steps, blocks = cover(a.time, block);
   int64_t splits = 1;
+  // Several of the narrow kernels' workgroups, with fewer registers, fit a compute unit: forward of
+  // 20 x 100000 x 7 float32 in 117 us by one, 85 by two, 83 by four.
+  const int64_t wanted = line || narrow ? 4 * kWorkgroups : kWorkgroups;
   if (a.groups < kWorkgroups * 7 / 16)
-    splits = std::min({cover(kWorkgroups, a.groups), blocks, kMostSplits});
+    splits = std::min({cover(wanted, a.groups), blocks, kMostSplits});
   a.split_steps = cover(blocks, splits) * block;
   a.splits = int32_t(cover(a.time, a.split_steps));
   a.streamed = across == 64 && a.batch_lanes >= 64 &&
