@@ -877,7 +877,7 @@ __global__ __launch_bounds__(WAVES * 64, row_waves(NV)) void row_kernel(Rows a) 
     if (counted && fabs(gap) < kNearBorder) {  // the whole workgroup agrees
       double sum = 0.0;
 #pragma unroll 1
-      for (int k = tid; k < k_all; k += team) sum += exact_element(float(row[k]), base);
+      for (int k = tid; k < k_all; k += team) sum += exact_element(float(row[k]), st.m);
       gap = exact_gap(a, in, zy, st.m, block_sum<team>(sum, part64));
       // Read again: the 64-bit code has their registers meanwhile.
 #pragma unroll
