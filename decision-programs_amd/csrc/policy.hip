@@ -46,20 +46,27 @@ __device__ __forceinline__ double log_sum(double s) {
   return double(e) * kLn2d + double(logf(float(f)));
 }
 
-// e^x - 1 - x without cancellation near 0.
-__device__ __forceinline__ float exp_minus_tangent(float x) {
-  if (fabsf(x) < 0.5f) {
-    float p = 1.0f / 362880.0f;
-    p = fmaf(p, x, 1.0f / 40320.0f);
-    p = fmaf(p, x, 1.0f / 5040.0f);
-    p = fmaf(p, x, 1.0f / 720.0f);
-    p = fmaf(p, x, 1.0f / 120.0f);
-    p = fmaf(p, x, 1.0f / 24.0f);
-    p = fmaf(p, x, 1.0f / 6.0f);
-    p = fmaf(p, x, 0.5f);
-    return x * x * p;
+// e^x - 1 and e^x - 1 - x.  Near 0 the second is a series, whose first term left out is below 1e-9
+// of it; from 0.5 on what cancels are a few of 64 bits.
+struct Growth {
+  double rise, bend;
+};
+
+__device__ __forceinline__ Growth growth(double x) {
+  if (fabs(x) < 0.5) {
+    double p = 1.0 / 362880.0;
+    p = fma(p, x, 1.0 / 40320.0);
+    p = fma(p, x, 1.0 / 5040.0);
+    p = fma(p, x, 1.0 / 720.0);
+    p = fma(p, x, 1.0 / 120.0);
+    p = fma(p, x, 1.0 / 24.0);
+    p = fma(p, x, 1.0 / 6.0);
+    p = fma(p, x, 0.5);
+    const double bend = x * x * p;
+    return {x + bend, bend};
   }
-  return (expf(x) - 1.0f) - x;
+  const double rise = exp(x) - 1.0;
+  return {rise, rise - x};
 }
 
 enum RowOp { kScore, kSlopes, kPolicy };
@@ -303,11 +310,11 @@ __device__ __forceinline__ void policy_row(const Rows& a, int64_t r, RowIn& in, 
   float c = active ? -plain : 0.0f;
   float kl = 0.0f;
   if (a.reference) {
-    const float d = float(double(in.reference) - o.logp);
-    kl = exp_minus_tangent(d);
+    const Growth g = growth(double(in.reference) - o.logp);
+    kl = float(g.bend);
     if (a.kl_weight != 0.0f) {
       loss = loss + a.kl_weight * kl;
-      c = c - a.kl_weight * (kl + d);
+      c = c - a.kl_weight * float(g.rise);  // -1 where the reference rules the action out
     }
   }
   if (a.entropy_weight != 0.0f) loss = loss - a.entropy_weight * o.h;

@@ -9,6 +9,9 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
+# rows of a thread, of some lanes, of a workgroup, in pieces (float32)
+WIDTHS = [4, 40, 5000, 40000]
+
 
 def _normal(*shape, key):
     import torch
@@ -31,6 +34,82 @@ def _logp(z, y):
     import torch
 
     return torch.log_softmax(z.double(), 1).gather(1, y[:, None])[:, 0]
+
+
+def _unlikely(n, k):
+    """Rows whose taken class has log-probability -70 exactly: exp(-70) is lost beside 1, also in
+    64 bits, and so is what its probability takes from its gradient."""
+    import torch
+
+    z = torch.full((n, k), -200.0, device="cuda")
+    y = torch.arange(n, device="cuda") % (k - 1)
+    z[:, k - 1] = 0.0
+    z.scatter_(1, y[:, None], -70.0)
+    return z, y
+
+
+# ---------------------------------------------------------------------------
+# The KL term
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("k", WIDTHS)
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_references_that_rule_the_action_out(ws, device, k, dtype):
+    """log-probability -infinity, or nearly: the estimate grows without bound, its slope is -1."""
+    import torch
+    from dpgbdt import ops
+
+    z, y = _rows(12, k, dtype)
+    logp = _logp(z, y)
+    reference = (logp - 0.1).float()
+    reference[::4] = -float("inf")
+    reference[1::4] = -1e8
+    reference[2::4] = -1e30
+    old, adv = logp.float(), torch.zeros(12, device="cuda")
+    out = ops.policy_loss(ws, z, y, old, adv, reference=reference, kl=0.5,
+                          hessian=dtype == "float32")
+    d = reference.double() - logp
+    far = torch.arange(12, device="cuda") % 4 != 3
+    assert torch.equal(out.kl[far], (-1.0 - d).float()[far])
+    assert torch.equal(out.loss[far], (0.5 * (-1.0 - d)).float()[far])
+    rows = ref64.Rows(z, y)
+    c = -0.5 * np.expm1(d.cpu().numpy())
+    # the slope: 0.5 of one rounding of e^d - 1, and of logp's error times e^d
+    slope = 0.5 * (2.0 ** -22 + np.exp(d.cpu().numpy()) * rows.logp_bound())
+    g, off = rows.grad(c, np.zeros(12))
+    ref64.close(out.grad, g, off + slope[:, None], "grad")
+    if out.hess is not None:
+        h, off = rows.hess(c, np.zeros(12))
+        ref64.close(out.hess, h, off + slope[:, None], "hess")
+
+
+@pytest.mark.parametrize("k", WIDTHS)
+def test_kl_term_to_its_last_bits(ws, device, k):
+    """e^d - 1 - d and e^d - 1 over the range of d, each to 2^-22 of itself: d is exact here (see
+    _unlikely), and each is a few roundings of 2^-24 away from its result."""
+    import torch
+    from dpgbdt import ops
+
+    size = torch.logspace(-3, np.log10(60.0), 32, device="cuda")
+    reference = torch.cat([size, -size, torch.tensor([0.5, -0.5, 1.0, -1.0], device="cuda")]) - 70.0
+    z, y = _unlikely(len(reference), k)
+    zero = torch.zeros_like(reference)
+    out = ops.policy_loss(ws, z, y, zero - 70.0, zero, reference=reference, kl=0.5)
+    d = reference.cpu().double().numpy() + 70.0
+    assert np.abs(d).max() > 59.0 and (d != 0).all()
+    want = np.where(np.abs(d) < 0.5, d * d * _tangent_rest(d), np.expm1(d) - d)
+    ref64.close(out.kl, want, 2.0 ** -22 * want, "kl")
+    ref64.close(out.loss, 0.5 * want, 2.0 ** -23 * want, "loss")
+    slope = 0.5 * np.expm1(d)
+    ref64.close(out.grad.gather(1, y[:, None])[:, 0], -slope, 2.0 ** -22 * np.abs(slope), "slope")
+
+
+def _tangent_rest(d):
+    """(e^d - 1 - d) / d^2 by its series, for |d| < 0.5."""
+    total, term = np.zeros_like(d), np.full_like(d, 0.5)
+    for i in range(3, 24):
+        total += term
+        term = term * d / i
+    return total
 
 
 # ---------------------------------------------------------------------------
