@@ -275,7 +275,7 @@ __device__ __forceinline__ float element_grad(float z, const RowSlopes& o, float
   const float g = p * fmaf(o.n2, fmaxf(x, kNoPower), o.a);
   if (HESS) {
     p *= o.corr;
-    hess = fmaxf(o.curve * (p * (1.0f - p)), o.least);
+    hess = __builtin_elementwise_maximum(o.curve * (p * (1.0f - p)), o.least);  // keeps NaN
   }
   return g;
 }

@@ -113,6 +113,33 @@ def _tangent_rest(d):
 
 
 # ---------------------------------------------------------------------------
+# NaN
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("k", WIDTHS)
+def test_hessians_keep_nan(ws, device, k):
+    import torch
+    from dpgbdt import ops
+
+    z, y = _rows(8, k)
+    old = _logp(z, y).float()
+    adv = torch.ones(8, device="cuda")
+    ptr = torch.tensor([0, 2, 4, 6, 8], device="cuda")
+    clean = ops.policy_loss(ws, z, y, old, adv, hessian=True)
+    pairs = ops.preference_loss(ws, z, y, ptr, hessian=True)
+    z[1, k // 2] = float("nan")
+    out = ops.policy_loss(ws, z, y, old, adv, hessian=True)
+    for x in out:
+        if x is not None:
+            assert x[1].isnan().all()
+    rest = [i for i in range(8) if i != 1]
+    assert torch.equal(out.hess[rest], clean.hess[rest])
+    out = ops.preference_loss(ws, z, y, ptr, hessian=True)
+    for x in (out.grad, out.hess):
+        assert x[:4].isnan().all()  # the pair's
+    assert torch.equal(out.grad[4:], pairs.grad[4:]) and torch.equal(out.hess[4:], pairs.hess[4:])
+
+
+# ---------------------------------------------------------------------------
 # The border of the clip
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("n,k,dtype", [(300, 9, "bfloat16"), (100, 1500, "float16"),
