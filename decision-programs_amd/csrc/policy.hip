@@ -307,7 +307,8 @@ __device__ __forceinline__ void policy_row(const Rows& a, int64_t r, RowIn& in, 
   const float plain = ratio * adv;
   const float clipped = fminf(fmaxf(ratio, a.low), a.high) * adv;
   float loss = -(plain < clipped || plain != plain ? plain : clipped);
-  float c = active ? -plain : 0.0f;
+  // Clipped: no slope.  NaN is on neither side of the border and stays.
+  float c = active || plain != plain ? -plain : 0.0f;
   float kl = 0.0f;
   if (a.reference) {
     const Growth g = growth(double(in.reference) - o.logp);

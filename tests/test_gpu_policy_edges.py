@@ -116,6 +116,40 @@ def _tangent_rest(d):
 # NaN
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("k", WIDTHS)
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("what", ["old", "advantage", "weight", "reference"])
+def test_nan_of_a_row_reaches_its_gradient(ws, device, k, dtype, what):
+    """On either side of either border of the clip, for advantages of either sign."""
+    import torch
+    from dpgbdt import ops
+
+    n = 16
+    z, y = _rows(n, k, dtype)
+    logp = _logp(z, y)
+    x = torch.tensor([-1.0, -0.3, -0.1, 0.0, 0.1, 0.3, 1.0, 2.0], device="cuda").repeat(2)
+    sign = torch.where(torch.arange(n, device="cuda") < 8, 1.0, -1.0)
+    args = {"old": (logp - x).float(), "advantage": sign, "weight": sign * 0 + 2.0,
+            "reference": (logp + 0.2).float()}
+
+    def loss(kl=0.1):
+        return ops.policy_loss(ws, z, y, args["old"], args["advantage"], args["weight"],
+                               args["reference"], kl=kl, hessian=dtype == "float32")
+
+    clean = loss()
+    bad = torch.arange(n, device="cuda") % 2 == 0
+    args[what] = torch.where(bad, float("nan"), args[what])
+    out = loss()
+    held = [out.loss, out.grad] + [out.hess] * (out.hess is not None)
+    for got, was in zip(held, [clean.loss, clean.grad, clean.hess]):
+        assert got[bad].isnan().all()
+        assert torch.equal(got[~bad], was[~bad])
+    if what == "reference":  # without the term's weight only its own output has it
+        out = loss(kl=0.0)
+        assert out.kl[bad].isnan().all() and not out.loss.isnan().any()
+        assert not out.grad.isnan().any()
+
+
+@pytest.mark.parametrize("k", WIDTHS)
 def test_hessians_keep_nan(ws, device, k):
     import torch
     from dpgbdt import ops
