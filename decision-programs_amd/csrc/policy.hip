@@ -302,9 +302,11 @@ __device__ __forceinline__ double exact_gap(const Rows& a, const RowIn& in, floa
 __device__ __forceinline__ void policy_row(const Rows& a, int64_t r, RowIn& in, const RowHead& o,
                                            double gap, bool write) {
   const float adv = in.advantage;
-  const float ratio = expf(float(o.logp - double(in.old_logp)));
+  const double log_ratio = o.logp - double(in.old_logp);
+  const float ratio = expf(float(log_ratio));
   const bool active = adv > 0.0f ? gap < 0.0 : gap > 0.0;
-  const float plain = ratio * adv;
+  // nothing times a ratio that is finite, if too large for its type
+  const float plain = adv == 0.0f && log_ratio < INFINITY ? 0.0f : ratio * adv;
   const float clipped = fminf(fmaxf(ratio, a.low), a.high) * adv;
   float loss = -(plain < clipped || plain != plain ? plain : clipped);
   // Clipped: no slope.  NaN is on neither side of the border and stays.

@@ -113,6 +113,28 @@ def _tangent_rest(d):
 
 
 # ---------------------------------------------------------------------------
+# The ratio
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("k", WIDTHS)
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_advantages_of_zero(ws, device, k, dtype):
+    """Nothing is lost or gained, however large the ratio."""
+    import torch
+    from dpgbdt import ops
+
+    z, y = _rows(8, k, dtype)
+    logp = _logp(z, y)
+    old = (logp - torch.tensor([0.0, 1.0, 88.0, 89.0, 100.0, 700.0, 800.0, 1e30],
+                               device="cuda")).float()
+    zero = torch.zeros(8, device="cuda")
+    for adv in (zero, -zero):
+        out = ops.policy_loss(ws, z, y, old, adv, hessian=dtype == "float32")
+        assert not out.loss.any() and not out.grad.any()
+        if out.hess is not None:
+            assert (out.hess == 1e-16).all()
+
+
+# ---------------------------------------------------------------------------
 # NaN
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("k", WIDTHS)
