@@ -46,27 +46,28 @@ __device__ __forceinline__ double log_sum(double s) {
   return double(e) * kLn2d + double(logf(float(f)));
 }
 
-// e^x - 1 and e^x - 1 - x.  Near 0 the second is a series, whose first term left out is below 1e-9
-// of it; from 0.5 on what cancels are a few of 64 bits.
+// e^x - 1 and e^x - 1 - x, to a rounding or two: x = k ln 2 + r, and the series of e^r, whose first
+// term left out is r^9 / 9! < 3e-10.  What is beside 1 + r in it is e^x - 1 - x for k = 0; for other
+// k what cancels are a few of 64 bits.  Beyond 200 e^x is beyond 32 bits.
 struct Growth {
-  double rise, bend;
+  float rise, bend;
 };
 
 __device__ __forceinline__ Growth growth(double x) {
-  if (fabs(x) < 0.5) {
-    double p = 1.0 / 362880.0;
-    p = fma(p, x, 1.0 / 40320.0);
-    p = fma(p, x, 1.0 / 5040.0);
-    p = fma(p, x, 1.0 / 720.0);
-    p = fma(p, x, 1.0 / 120.0);
-    p = fma(p, x, 1.0 / 24.0);
-    p = fma(p, x, 1.0 / 6.0);
-    p = fma(p, x, 0.5);
-    const double bend = x * x * p;
-    return {x + bend, bend};
-  }
-  const double rise = exp(x) - 1.0;
-  return {rise, rise - x};
+  x = x > 200.0 ? 200.0 : x;  // NaN stays
+  const double held = x < -200.0 ? -200.0 : x;
+  const double k = rint(held * 1.4426950408889634);
+  const double r = fma(-k, kLn2d, held);
+  double q = 1.0 / 40320.0;
+  q = fma(q, r, 1.0 / 5040.0);
+  q = fma(q, r, 1.0 / 720.0);
+  q = fma(q, r, 1.0 / 120.0);
+  q = fma(q, r, 1.0 / 24.0);
+  q = fma(q, r, 1.0 / 6.0);
+  q = fma(q, r, 0.5);
+  const double beside = r * r * q, scale = ldexp(1.0, int(k));
+  const double rise = fma(scale, r + beside, scale - 1.0);
+  return {float(rise), float(k == 0.0 ? beside : rise - x)};
 }
 
 enum RowOp { kScore, kSlopes, kPolicy };
@@ -314,10 +315,10 @@ __device__ __forceinline__ void policy_row(const Rows& a, int64_t r, RowIn& in, 
   float kl = 0.0f;
   if (a.reference) {
     const Growth g = growth(double(in.reference) - o.logp);
-    kl = float(g.bend);
+    kl = g.bend;
     if (a.kl_weight != 0.0f) {
       loss = loss + a.kl_weight * kl;
-      c = c - a.kl_weight * float(g.rise);  // -1 where the reference rules the action out
+      c = c - a.kl_weight * g.rise;  // -1 where the reference rules the action out
     }
   }
   if (a.entropy_weight != 0.0f) loss = loss - a.entropy_weight * o.h;
