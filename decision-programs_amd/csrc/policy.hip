@@ -46,6 +46,13 @@ __device__ __forceinline__ double log_sum(double s) {
   return double(e) * kLn2d + double(logf(float(f)));
 }
 
+// e^x with what x loses in 32 bits put right.
+__device__ __forceinline__ float exp_of(double x) {
+  const float most = float(x);
+  const float e = expf(most);
+  return fabsf(most) < 88.0f ? fmaf(e, float(x - double(most)), e) : e;
+}
+
 // e^x - 1 and e^x - 1 - x, to a rounding or two: x = k ln 2 + r, and the series of e^r, whose first
 // term left out is r^9 / 9! < 3e-10.  What is beside 1 + r in it is e^x - 1 - x for k = 0; for other
 // k what cancels are a few of 64 bits.  Beyond 200 e^x is beyond 32 bits.
@@ -304,7 +311,7 @@ __device__ __forceinline__ void policy_row(const Rows& a, int64_t r, RowIn& in, 
                                            double gap, bool write) {
   const float adv = in.advantage;
   const double log_ratio = o.logp - double(in.old_logp);
-  const float ratio = expf(float(log_ratio));
+  const float ratio = exp_of(log_ratio);
   const bool active = adv > 0.0f ? gap < 0.0 : gap > 0.0;
   // nothing times a ratio that is finite, if too large for its type
   const float plain = adv == 0.0f && log_ratio < INFINITY ? 0.0f : ratio * adv;

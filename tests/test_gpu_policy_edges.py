@@ -116,6 +116,25 @@ def _tangent_rest(d):
 # The ratio
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("k", WIDTHS)
+def test_ratio_to_its_last_bits(ws, device, k):
+    """Log-ratios that 32 bits do not hold, of both signs: loss and slope are two roundings away
+    from the ratio of exact numbers (see _unlikely)."""
+    import torch
+    from dpgbdt import ops
+
+    old = -torch.cat([torch.linspace(0.3, 20.0, 40, device="cuda"),
+                      torch.linspace(70.3, 130.0, 40, device="cuda")])
+    z, y = _unlikely(len(old), k)
+    x = -70.0 - old.cpu().double().numpy()
+    assert (np.float32(x) != x).sum() > 30
+    adv = torch.where(old > -70.0, 1.5, -1.5)  # the side on which nothing is clipped
+    out = ops.policy_loss(ws, z, y, old, adv)
+    want = -np.exp(x) * adv.cpu().double().numpy()
+    ref64.close(out.loss, want, 2.0 ** -23 * np.abs(want), "loss")
+    ref64.close(out.grad.gather(1, y[:, None])[:, 0], want, 2.0 ** -22 * np.abs(want), "slope")
+
+
+@pytest.mark.parametrize("k", WIDTHS)
 @pytest.mark.parametrize("dtype", ["float32", "float16"])
 def test_advantages_of_zero(ws, device, k, dtype):
     """Nothing is lost or gained, however large the ratio."""
