@@ -1282,8 +1282,11 @@ __device__ __forceinline__ void one_pair(const Pairs& a, int64_t pair, const Pai
   }
   if (tid == 0) {
     const double l = log1p(q);  // -log sigma(|score|)
-    a.loss[pair] = float((1.0 - a.smoothing) * (l + fmax(-score, 0.0)) +
-                         a.smoothing * (l + fmax(score, 0.0)));
+    // An infinite score has a term that is infinite; without weight it adds nothing.
+    double loss = 0.0;
+    if (a.smoothing < 1.0) loss += (1.0 - a.smoothing) * (l + fmax(-score, 0.0));
+    if (a.smoothing > 0.0) loss += a.smoothing * (l + fmax(score, 0.0));
+    a.loss[pair] = float(loss);
     if (a.score) a.score[pair] = float(score);
   }
 }

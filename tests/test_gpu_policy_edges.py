@@ -215,6 +215,34 @@ def test_hessians_keep_nan(ws, device, k):
 
 
 # ---------------------------------------------------------------------------
+# Certain preferences
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [3, 400])
+@pytest.mark.parametrize("smoothing", [0.0, 1.0, 0.25])
+def test_pairs_with_an_illegal_action(ws, device, rows, smoothing):
+    """The scores are infinite; a term without weight adds nothing, and no gradient is lost."""
+    import torch
+    from dpgbdt import ops
+
+    n, beta = 4 * rows, 0.5
+    z, y = _rows(n, 10)
+    for at in (rows + 1, 2 * rows + 1):  # in the first pair's worse, the second's better sequence
+        z[at, y[at]] = -float("inf")
+    ptr = torch.arange(0, n + 1, rows, device="cuda")
+    out = ops.preference_loss(ws, z, y, ptr, beta=beta, smoothing=smoothing, hessian=True)
+    inf = float("inf")
+    assert out.score.tolist() == [inf, -inf]
+    assert out.loss.tolist() == [inf if smoothing > 0.0 else 0.0, inf if smoothing < 1.0 else 0.0]
+    slope = np.array([smoothing, -(1.0 - smoothing)]) * beta  # the limits of the sigmoids
+    c = np.repeat(np.stack([slope, -slope], 1).ravel(), rows)
+    reference = ref64.Rows(z, y)
+    g, off = reference.grad(c, np.zeros(n))
+    ref64.close(out.grad, g, off, "grad")
+    h, off = reference.hess(c, np.zeros(n))
+    ref64.close(out.hess, h, off, "hess")
+
+
+# ---------------------------------------------------------------------------
 # The border of the clip
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("n,k,dtype", [(300, 9, "bfloat16"), (100, 1500, "float16"),
