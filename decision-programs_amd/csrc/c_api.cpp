@@ -192,13 +192,18 @@ void dp_workspace_s::reserve_scratch(size_t bytes) {
   if (bytes > scratch.n) {
     size_t cap = 1 << 20;
     while (cap < bytes) cap <<= 1;
-    scratch.resize(cap);
+    if (!in_graphs_) return scratch.resize(cap);
+    dp::DeviceBuffer<uint8_t> larger(cap);
+    outgrown_.push_back(std::move(scratch));
+    scratch = std::move(larger);
+    in_graphs_ = false;
   }
 }
 
 uint8_t* dp_workspace_s::scratch_only(size_t bytes) {
   scratch_used = 0;
   reserve_scratch(bytes);
+  if (bytes) in_graphs_ = true;
   return scratch.p;
 }
 

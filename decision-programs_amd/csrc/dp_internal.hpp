@@ -275,10 +275,14 @@ struct dp_workspace_s {
   void reserve_scratch(size_t bytes);
   // Device-only scratch for a call that stages nothing: no host wait and no
   // event, so that a call whose scratch is large enough already can be captured
-  // into a graph.
+  // into a graph.  A graph goes on using the block that it was captured with, so
+  // a block handed out here lives as long as the workspace, also when a larger
+  // one takes its place (blocks double: together they are less than the last).
   uint8_t* scratch_only(size_t bytes);
 
  private:
+  bool in_graphs_ = false;  // scratch has been handed out by scratch_only
+  std::vector<dp::DeviceBuffer<uint8_t>> outgrown_;
   std::vector<uint8_t> committed_;  // the bytes the device staging area holds
   void grow_staging(size_t bytes);
   [[noreturn]] void need_scratch(size_t bytes);

@@ -44,7 +44,8 @@ def _ptr(t):
 
 
 class Workspace:
-    """Device scratch reused by the operator entry points."""
+    """Device scratch reused by the operator entry points, by one stream at a time.  A graph that
+    calls were captured into uses it at every replay: keep it as long as the graph."""
 
     def __init__(self):
         self.handle = c_void_p()

@@ -384,7 +384,11 @@ int dp_update_margin(dp_workspace ws, const uint32_t* ridx, const int64_t* begin
  * over 8 classes); the same call gives the same bits every time, and log p_y of
  * the same margins is the same in every call.  Any row stride will do.
  * The calls allocate nothing once the workspace has grown to their size, and can
- * be captured into a graph then.  Use one stream at a time per workspace. */
+ * be captured into a graph then.  A graph uses the workspace's scratch whenever it
+ * is replayed: keep the workspace until the graph's last replay has ended, and
+ * count a replay as a use of it by the stream that it runs on.  Larger calls may
+ * follow (their scratch does not replace what a graph uses).  Use one stream at a
+ * time per workspace. */
 enum dp_dtype { DP_FLOAT32 = 0, DP_FLOAT16 = 1, DP_BFLOAT16 = 2 };
 
 typedef struct {

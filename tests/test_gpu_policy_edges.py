@@ -272,3 +272,51 @@ def test_border_of_the_clip_in_every_kernel(ws, device, n, k, dtype):
     slope = np.abs(c) * 2.0 ** -20  # logp's error and roundings of the ratio
     some = np.flatnonzero(clear)
     ref64.close(out.grad[some], g[some], (off + slope[:, None])[some], "grad")
+
+
+# ---------------------------------------------------------------------------
+# Graphs
+# ---------------------------------------------------------------------------
+def test_graphs_outlive_a_growth_of_the_workspace(device):
+    """Larger calls between the replays take other scratch; memory that is allocated after them is
+    not what the graph writes to."""
+    import torch
+    from dpgbdt import ops
+
+    ws = ops.Workspace()
+    z, y = _rows(40, 40000)  # rows in pieces
+    few, act = _rows(3000, 10)
+    ptr = torch.arange(0, 3001, 100, device="cuda")
+    gate = torch.sigmoid(_normal(1, 40000, 64, key="gate") + 3.0)  # in splits
+    value = _normal(1, 40000, 64, key="value")
+
+    def calls():
+        state, last = ops.linear_recurrence(ws, gate, value)
+        back = ops.linear_recurrence_backward(ws, gate, state, value)
+        out = [state, last, *back, *ops.action_logprobs(ws, z, y, entropy=True),
+               *ops.preference_loss(ws, few, act, ptr),
+               *ops.preference_loss(ws, z, y, ptr[:3] // 10)]
+        return [x for x in out if x is not None]
+
+    calls()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = calls()
+    many, acts = _rows(1 << 21, 4)
+    marks = []
+    for i in range(4):
+        n = len(many) >> (3 - i)  # each larger than any before
+        pairs = torch.tensor([0, n // 2, n], device="cuda")
+        ops.preference_loss(ws, many[:n], acts[:n], pairs)
+        torch.cuda.synchronize()
+        marks += [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(64)]
+        for x in outs:
+            x.zero_()
+        value.mul_(-1.0)
+        few.add_(0.125)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = calls()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
+    assert all((x == 7.0).all() for x in marks)
