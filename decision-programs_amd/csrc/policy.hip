@@ -1230,6 +1230,7 @@ Rows rows_of(const dp_decisions& d) {
 struct Pairs {
   const int64_t* sequences;
   int64_t n_pairs, n_rows;
+  int64_t first;  // pair of the launch's first workgroup
   const double* logp;  // kNotCounted: the row is not
   const float* reference;
   double beta, smoothing;
@@ -1307,7 +1308,7 @@ __global__ __launch_bounds__(kThreads) void pair_kernel(Pairs a, int lanes) {
   __shared__ int64_t left[kThreads];
   const int team = int(threadIdx.x) / lanes, tid = int(threadIdx.x) & (lanes - 1);
   const int teams = kThreads / lanes;
-  const int64_t pair = int64_t(blockIdx.x) * teams + team;
+  const int64_t pair = a.first + int64_t(blockIdx.x) * teams + team;
   const bool live = pair < a.n_pairs;
   PairRows at{};
   if (live) at = pair_rows(a, pair);
@@ -1325,8 +1326,7 @@ __global__ __launch_bounds__(kThreads) void pair_kernel(Pairs a, int lanes) {
                [&](double v) { return block_sum<kThreads>(v, part); });
 }
 
-// n_pairs < 2^31: fewer than 2^32 threads below.
-void launch_pairs(const Pairs& q, hipStream_t s) {
+void launch_pairs(Pairs q, hipStream_t s) {
   const int64_t rows = q.n_rows / q.n_pairs;
   if (rows >= 4 * 64 && q.n_pairs < (1 << 20)) {
     long_pair_kernel<<<unsigned(q.n_pairs), kThreads, 0, s>>>(q);
@@ -1334,8 +1334,10 @@ void launch_pairs(const Pairs& q, hipStream_t s) {
     // About two rows of a pair a lane.
     int lanes = 1;
     while (lanes < 64 && lanes * 2 < rows) lanes *= 2;
-    const int64_t teams = kThreads / lanes;
-    pair_kernel<<<unsigned((q.n_pairs + teams - 1) / teams), kThreads, 0, s>>>(q, lanes);
+    in_launches(q.n_pairs, kThreads / lanes, [&](int64_t first, unsigned n) {
+      q.first = first;
+      pair_kernel<<<n, kThreads, 0, s>>>(q, lanes);
+    });
   }
   DP_HIP(hipGetLastError());
 }

@@ -1,7 +1,13 @@
 """What the operators over decisions hold and launch, without a GPU: on a HIP runtime in host
 memory, whose kernels do nothing."""
+import json
+import os
+import subprocess
+import sys
+import textwrap
+
 import pytest
-from test_host_memory import host  # noqa: F401  (fixture)
+from test_host_memory import HERE, PRELUDE, host  # noqa: F401  (fixture)
 from test_policy_refusals import SETUP
 
 CALLS = """
@@ -72,3 +78,55 @@ def test_a_growth_that_finds_no_memory_leaves_the_scratch(host):  # noqa: F811
     print(json.dumps([failed, live() - before]))
     """)
     assert got[0] != 0 and got[1] == 0
+
+
+# Allocations of the runtime in host memory take address space only: the scratch of very many
+# rows, which no kernel touches there.
+RESERVE = """
+#include <cstdlib>
+#include <sys/mman.h>
+namespace std {
+inline void* reserve(size_t count, size_t bytes) {
+  void* p = mmap(nullptr, count * bytes, PROT_READ | PROT_WRITE,
+                 MAP_PRIVATE | MAP_ANONYMOUS | MAP_NORESERVE, -1, 0);
+  return p == MAP_FAILED ? nullptr : p;
+}
+}
+#define calloc reserve
+"""
+
+
+@pytest.fixture(scope="session")
+def vast(dp, tmp_path_factory):
+    """Runs code as `host` does, with allocations of any size."""
+    folder = tmp_path_factory.mktemp("vast")
+    header, fake = folder / "reserve.hpp", folder / "libfake_hip.so"
+    header.write_text(RESERVE)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__",
+                    "-I/opt/rocm/include", "-include", str(header), "-o", str(fake),
+                    os.path.join(HERE, "native", "fake_hip.cpp")], check=True)
+
+    def run(code):
+        text = PRELUDE.format(fake=str(fake), lib=dp.LIB_PATH) + textwrap.dedent(code)
+        p = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True,
+                           timeout=120)
+        assert p.returncode == 0, p.stderr
+        return json.loads(p.stdout)
+
+    return run
+
+
+@pytest.mark.parametrize("pairs,rows,lanes", [(2 ** 31 - 1, 0, 1), (2 ** 31 - 1, 3, 2),
+                                              (1 << 30, 5, 4), (1 << 26, 65, 64), (5000, 3, 2)])
+def test_pairs_are_launched_in_parts_that_a_grid_holds(vast, pairs, rows, lanes):
+    """A launch has fewer than 2^32 threads, also where each of very many pairs takes several."""
+    got = vast(SETUP + f"""
+    ok(lib.dp_preference_loss(ws, rows(n_rows={pairs * rows}, n_classes=1, row_stride=1, dtype=1),
+                              P, c_int64({pairs}), None, byref(Preference(0.1, 0.0, 0)), P, None,
+                              None, P, None, None))
+    seen = [x.split(" ") for x in fake.fake_launches().decode().split(";") if x]
+    print(json.dumps([[n, int(g.split(",")[0]), int(b)] for n, g, b in seen]))
+    """)
+    assert all(grid * block < 2 ** 32 for _, grid, block in got)
+    threads = sum(grid * block for name, grid, block in got if "pair_kernel" in name)
+    assert 0 <= threads - lanes * pairs < 256
