@@ -47,7 +47,7 @@ def _case(k, dtype, n=None, illegal=0.0, scale=2.0):
     g = _rng(k, dtype, n, illegal)
     z, y = _margins(g, n, k, dtype, scale, illegal)
     lp = torch.log_softmax(z.double(), 1).gather(1, y[:, None])[:, 0]
-    # 0.1 and more away from every border: which side is not in doubt (see the border test)
+    # on any side of the clip's borders (rows next to one: the border tests)
     old = (lp - torch.randn(n, generator=g, device="cuda") * 0.15).float()
     reference = (lp + torch.randn(n, generator=g, device="cuda") * 0.2).float()
     adv = torch.randn(n, generator=g, device="cuda")

@@ -243,6 +243,130 @@ def test_pairs_with_an_illegal_action(ws, device, rows, smoothing):
 
 
 # ---------------------------------------------------------------------------
+# Rows read twice by a workgroup: 256 and more, longer than 128 KB
+# ---------------------------------------------------------------------------
+LONG = [("float32", 33001), ("bfloat16", 65601), ("float16", 65601)]
+
+
+def _long(dtype, k, n=257):
+    """Margins with an illegal class in ten, rows that are not counted, rows without a class."""
+    import torch
+
+    z, y = _rows(n, k, dtype)
+    illegal = _normal(n, k, key="illegal") < -1.28
+    illegal.scatter_(1, y[:, None], False)
+    z.masked_fill_(illegal, -float("inf"))
+    y[5::50] = -1
+    y[6::50] = k
+    z[5::50] = z[6::50] = float("nan")
+    z[7::50] = -float("inf")
+    y[8], y[9] = k - 1, 0
+    z[8, k - 1] = z[9, 0] = 1.0
+    return z, y
+
+
+@pytest.mark.parametrize("dtype,k", LONG)
+def test_long_rows_of_many(ws, device, dtype, k):
+    import torch
+    from dpgbdt import ops
+
+    z, y = _long(dtype, k)
+    n = len(y)
+    rows = ref64.Rows(z, y)
+    logp, h = ops.action_logprobs(ws, z, y, entropy=True)
+    ref64.close(logp, rows.keep(rows.logp), rows.logp_bound(), "logp")
+    ref64.close(h, rows.keep(rows.h), rows.h_bound(), "entropy")
+    dlogp, dent = _normal(n, key="dlogp"), _normal(n, key="dentropy")
+    grad = ops.action_logprobs_backward(ws, z, y, dlogp, dent)
+    g, off = rows.grad(rows.keep(dlogp.cpu().double().numpy()),
+                       rows.keep(-dent.cpu().double().numpy()))
+    ref64.close(grad, g, off, "backward")
+
+
+def _policy_inputs(z, y):
+    import torch
+
+    n, k = z.shape
+    logp = _logp(torch.nan_to_num(z, 0.0, neginf=-300.0), y.clamp(0, k - 1))
+    x = _normal(n, key="x") * 0.4
+    x = torch.where((x - 0.2).abs() < 0.05, x - 0.1, x)     # off the borders
+    x = torch.where((x + 0.22).abs() < 0.05, x + 0.1, x)
+    return ((logp - x).float(), _normal(n, key="adv"), _normal(n, key="w").abs() + 0.5,
+            (logp + _normal(n, key="ref") * 0.2).float())
+
+
+@pytest.mark.parametrize("dtype,k", LONG)
+def test_long_rows_of_many_policy(ws, device, dtype, k):
+    from dpgbdt import ops
+
+    z, y = _long(dtype, k)
+    old, adv, weight, reference = _policy_inputs(z, y)
+    weight[3::50] = 0.0
+    out = ops.policy_loss(ws, z, y, old, adv, weight, reference, kl=0.05, entropy=0.01,
+                          hessian=dtype == "float32")
+    _check_policy(out, z, y, old, adv, weight, reference, 0.05, 0.01)
+    if out.hess is not None:
+        plain = ops.policy_loss(ws, z, y, old, adv, weight, reference, kl=0.05, entropy=0.01)
+        assert (plain.grad == out.grad).all()
+
+
+def _check_policy(out, z, y, old, adv, weight, reference, kl, entropy):
+    rows = ref64.Rows(z, y, weight)
+    loss, k3, c, n = ref64.policy(rows, old, adv, reference, 0.2, 0.2, kl, entropy)
+    off = rows.logp_bound()
+    a = np.abs(adv.cpu().double().numpy())
+    ratio = np.exp(np.where(rows.counted, rows.logp - old.cpu().double().numpy(), 0.0))
+    ed = np.exp(np.where(rows.counted, reference.cpu().double().numpy() - rows.logp, 0.0))
+    ref64.close(out.logp, rows.keep(rows.logp), off, "logp")
+    ref64.close(out.entropy, rows.keep(rows.h), rows.h_bound(), "entropy")
+    k_off = rows.keep(np.abs(ed - 1.0) * off + 1e-12)  # the second order in logp's error
+    ref64.close(out.kl, k3, k_off + np.abs(k3) * 2.0 ** -22, "kl")
+    slope = rows.keep(rows.w * (a * ratio * (off + 2.0 ** -22) + kl * (ed * off + 2.0 ** -22)))
+    loss_off = rows.w * (a * np.maximum(ratio, 1.2) * (off + 2.0 ** -22) + kl * k_off
+                         + entropy * rows.h_bound())
+    ref64.close(out.loss, loss, rows.keep(loss_off) + np.abs(loss) * 2.0 ** -22, "loss")
+    g, g_off = rows.grad(c, n)
+    ref64.close(out.grad, g, g_off + slope[:, None], "grad")
+    if out.hess is not None:
+        h, h_off = rows.hess(c, n)
+        ref64.close(out.hess, h, h_off + slope[:, None], "hess")
+
+
+@pytest.mark.parametrize("dtype,k", LONG)
+@pytest.mark.parametrize("average", [False, True])
+def test_long_rows_of_many_preference(ws, device, dtype, k, average):
+    """Statistics are kept from the scores for the gradient."""
+    import torch
+    from dpgbdt import ops
+
+    z, y = _long(dtype, k)
+    n, beta = len(y), 0.02
+    ptr = torch.tensor([0, 30, 50, 50, 120, 200, 250], device="cuda")  # the last rows: of no pair
+    reference = _normal(n, key="ref") * 0.1 - 11.0
+    out = ops.preference_loss(ws, z, y, ptr, reference, beta=beta, smoothing=0.1, average=average,
+                              hessian=dtype == "float32")
+    rows = ref64.Rows(z, y)
+    score, loss, c = ref64.preference(rows, ptr, reference, beta, 0.1, average)
+    off = rows.logp_bound()
+    edges = ptr.cpu().numpy()
+    count = np.array([rows.counted[b:e].sum() for b, e in zip(edges, edges[1:])])
+    share = 1.0 / np.maximum(count, 1) if average else np.ones(6)
+    sums = np.array([off[b:e].sum() for b, e in zip(edges, edges[1:])]) * share
+    s_off = beta * (sums[0::2] + sums[1::2])
+    ref64.close(out.logp, rows.keep(rows.logp), off, "logp")
+    ref64.close(out.score, score, s_off, "score")
+    ref64.close(out.loss, loss, s_off + 2.0 ** -24, "loss")
+    slope = np.zeros(n)
+    for i in range(6):
+        slope[edges[i]:edges[i + 1]] = beta * s_off[i // 2] * share[i]
+    g, g_off = rows.grad(c, np.zeros(n))
+    ref64.close(out.grad, g, g_off + rows.keep(slope)[:, None], "grad")
+    if out.hess is not None:
+        h, h_off = rows.hess(c, np.zeros(n))
+        ref64.close(out.hess, h, h_off + rows.keep(slope)[:, None], "hess")
+
+
+# ---------------------------------------------------------------------------
 # The border of the clip
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("n,k,dtype", [(300, 9, "bfloat16"), (100, 1500, "float16"),
