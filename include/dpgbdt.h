@@ -381,8 +381,13 @@ int dp_update_margin(dp_workspace ws, const uint32_t* ridx, const int64_t* begin
  * gradient 0; a row with no other class is not counted either.  NaN in a counted
  * row reaches that row's outputs only (and its pair's).  Sums of exponentials,
  * log p_y and its differences are held in 64 bits (sums of 16-bit margins in 32
- * over 8 classes); the same call gives the same bits every time, and log p_y of
- * the same margins is the same in every call.  Any row stride will do.
+ * over 8 classes); exponentials, the logarithm of a sum and what a loss is put
+ * together from are rounded to 32 bits.  The same call gives the same bits every
+ * time.  log p_y and H of a row of at most 8192 whole vectors of 16 bytes are the
+ * same bits in every call.  Longer rows are added up in pieces that go by the
+ * number of rows: theirs are the same in all calls of as many rows, and equal to
+ * rounding in others.  Any row stride will do; outputs overlap neither inputs nor
+ * each other.
  * The calls allocate nothing once the workspace has grown to their size, and can
  * be captured into a graph then.  A graph uses the workspace's scratch whenever it
  * is replayed: keep the workspace until the graph's last replay has ended, and
@@ -446,8 +451,10 @@ typedef struct {
  * counted rows (reference NULL: 0), in 64 bits:
  *   score = beta (S of 2 i - S of 2 i + 1)
  *   loss = -(1 - smoothing) log sigma(score) - smoothing log sigma(-score)
+ * A term whose weight is 0 adds nothing, also where its logarithm is infinite.
  * logp [n_rows], score [n_pairs], grad and hess as in dp_policy_loss (rows of no
- * sequence: 0); all four may be NULL. */
+ * sequence have slope 0: gradient 0 and, if counted, hessian 1e-16); all four may
+ * be NULL. */
 int dp_preference_loss(dp_workspace ws, const dp_decisions* decisions, const int64_t* sequences,
                        int64_t n_pairs, const float* reference, const dp_preference_param* param,
                        float* loss, float* score, float* logp, void* grad, float* hess,
@@ -459,7 +466,9 @@ int dp_preference_loss(dp_workspace ws, const dp_decisions* decisions, const int
  * gamma * lambda where the episode goes on and 0 where it ends).  Element
  * (b, t, c) of array i is at b * strides[i][0] + t * strides[i][1] + c.  States
  * are held in 32 bits.  Products of gates over a span are formed, so they must
- * not overflow (gates of at most 1 in size never do). */
+ * not overflow (gates of at most 1 in size never do).  After a state that is not
+ * finite the later ones of its column are not either (infinite or NaN); others are
+ * not touched.  Outputs overlap neither inputs nor each other. */
 typedef struct {
   int64_t batch, time, channels;
   int32_t dtype;   /* dp_dtype of all arrays but initial, last, dlast, dinitial (float) */

@@ -399,6 +399,42 @@ def test_border_of_the_clip_in_every_kernel(ws, device, n, k, dtype):
 
 
 # ---------------------------------------------------------------------------
+# The same margins in other calls
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,k", [("float32", 7), ("float32", 100), ("bfloat16", 700),
+                                     ("float32", 5000), ("float32", 32771), ("float16", 65543)])
+def test_log_probabilities_do_not_go_by_the_batch(ws, device, dtype, k):
+    """Rows of up to 8192 whole vectors of 16 bytes: the same bits whatever is beside them."""
+    import torch
+    from dpgbdt import ops
+
+    z, y = _rows(300, k, dtype)
+    logp, h = ops.action_logprobs(ws, z, y, entropy=True)
+    for first, n in ((0, 1), (3, 24), (17, 255), (40, 256)):
+        zz, yy = z[first:first + n], y[first:first + n]
+        some, hh = ops.action_logprobs(ws, zz, yy, entropy=True)
+        assert torch.equal(some, logp[first:first + n]) and torch.equal(hh, h[first:first + n])
+        out = ops.policy_loss(ws, zz, yy, some, some, hessian=dtype == "float32")
+        assert torch.equal(out.logp, some) and torch.equal(out.entropy, hh)
+
+
+@pytest.mark.parametrize("dtype,k", [("float32", 40000), ("bfloat16", 90001)])
+@pytest.mark.parametrize("n", [1, 24, 255, 256])
+def test_log_probabilities_of_long_rows_go_by_the_row_count_only(ws, device, dtype, k, n):
+    import torch
+    from dpgbdt import ops
+
+    z, y = _rows(n, k, dtype)
+    logp, h = ops.action_logprobs(ws, z, y, entropy=True)
+    out = ops.policy_loss(ws, z, y, logp, logp, hessian=dtype == "float32")
+    assert torch.equal(out.logp, logp) and torch.equal(out.entropy, h)
+    pairs = ops.preference_loss(ws, z, y, torch.tensor([0, n // 2, n], device="cuda"))
+    assert torch.equal(pairs.logp, logp)
+    rows = ref64.Rows(z, y)
+    ref64.close(logp, rows.logp, rows.logp_bound(), "logp")
+
+
+# ---------------------------------------------------------------------------
 # Graphs
 # ---------------------------------------------------------------------------
 def test_graphs_outlive_a_growth_of_the_workspace(device):
