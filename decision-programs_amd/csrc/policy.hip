@@ -11,13 +11,16 @@
 // A class whose margin is -infinity has probability zero and adds nothing; a row
 // without any other class is not counted.
 //
-// Exponentials are 32-bit; their sums, log p_y, its differences to old and reference
-// log-probabilities and the sums over sequences are held in 64 bits: the difference
-// of two log-probabilities of about -10 that differ by 0.1 keeps 5 digits in 32.
+// Held in 64 bits: sums of exponentials, log p_y, its differences to old and reference
+// log-probabilities (the difference of two of about -10 that differ by 0.1 keeps 5 digits in
+// 32), e^d - 1 - d and the sums over sequences.  In 32 bits, since each is a rounding beside those
+// of the outputs: an element's exponential, of which a sum has the mean error; the logarithm
+// of a sum; sum e^d d, and the entropy with it; the ratio; what a loss and its slopes are
+// put together from.
 //
-// All kernels are bound by HBM where there is work for the whole chip, so each row is
-// read once if it can be held: in LDS and a thread's registers (short rows), in the
-// registers of some lanes, of a wave or of a workgroup.  Times below are of one MI355X,
+// Bound by HBM where there is work for the whole chip (16-bit rows of up to 512 vectors: by
+// vector instructions), so each row is read once if it can be held: in LDS and a thread's
+// registers (short rows), in the registers of some lanes, of a wave or of a workgroup.  Times below are of one MI355X,
 // where a large copy moves 4.8 TB/s.
 #include <algorithm>
 #include <cmath>
@@ -37,7 +40,7 @@ constexpr double kLog2eLoss = 1.0 - double(kLog2e) * kLn2d;
 // Below this power of two everything is 0.
 constexpr float kNoPower = -200.0f;
 
-// log s, to about 2^-25 of itself: s is at least 1 but for roundings, so that a sum near 1, of
+// log s, to about 2^-23 of itself: s is at least 1 but for roundings, so that a sum near 1, of
 // a row that one class has almost all of, goes by what is beside that 1.
 __device__ __forceinline__ double log_sum(double s) {
   if (s < 2.0) return double(log1pf(float(s - 1.0)));
@@ -256,7 +259,9 @@ __device__ __forceinline__ RowHead row_head(const Stats& st, float zy) {
 
 // What the gradient's elements take of their row:
 //   x = (z - m) kLog2e - log2 s,  p = 2^x corr,  gradient p (n (x ln 2 + H) - c) + [taken] c
-// corr holds what log2 s loses in 32 bits; n2 and a hold the row's slopes times corr.
+// corr holds what log2 s loses in 32 bits; n2 and a hold the row's slopes times corr.  x is rounded
+// once, to 2^-24 of itself: |log p| 2^-24 of p.  What kLog2e loses is a quarter of the rounding of
+// z - m and stays here (a gradient adds up over no sequence).
 struct RowSlopes {
   float m, log2_s, corr, n2, a, c, curve, least;
 };

@@ -480,3 +480,46 @@ def test_graphs_outlive_a_growth_of_the_workspace(device):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
     assert all((x == 7.0).all() for x in marks)
+
+
+# ---------------------------------------------------------------------------
+# How exact
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("k", [10, 40, 1000, 5000, 40000])
+def test_gradients_by_the_roundings_they_have(ws, device, k):
+    """p: z - m and the exponent are rounded once each, |z - m| and |log p| times 2^-24; the
+    hardware's 2^x to 2^-23; its products and the slope six times 2^-24.  The sum of exponentials
+    has the mean of what its terms are off by."""
+    from dpgbdt import ops
+
+    z, y = _rows(64, k, scale=3.0)
+    dlogp = _normal(64, key="dlogp")
+    grad = ops.action_logprobs_backward(ws, z, y, dlogp)
+    rows = ref64.Rows(z, y)
+    c = dlogp.cpu().double().numpy()[:, None]
+    mean = (rows.p * rows.d).sum(1, keepdims=True)
+    rel = (1.25 * rows.d + np.abs(rows.lp) + 1.25 * mean + 2.0 + 2.0 + 6.0) * 2.0 ** -24
+    taken = np.zeros_like(rows.p)
+    taken[np.arange(64), rows.y] = 1.0
+    want = c * (taken - rows.p)
+    ref64.close(grad, want, np.abs(c) * rows.p * rel + np.abs(want) * 2.0 ** -24
+                + np.abs(c) * taken * 2.0 ** -24, "grad")
+
+
+def test_log_probabilities_of_a_sequence_have_no_common_error(ws, device):
+    """What all rows are off by in the same way adds up over a sequence.  log2(e) loses 1.3e-8 of
+    itself in 32 bits; by 0.8 of probability at e^-10.4 it would be 1.1e-7 a row, against the 2^-25
+    that the hardware's exponential may be biased by and the 2^-25 of everything else."""
+    import torch
+    from dpgbdt import ops
+
+    n, k = 300, 130000
+    z = _normal(n, k, key="bias") * 0.25 - float(np.log(k / 4.0))
+    y = torch.zeros(n, dtype=torch.int64, device="cuda")
+    z[:, 0] = 0.0
+    logp = torch.cat([_logp(z[i:i + 50], y[i:i + 50]) for i in range(0, n, 50)])
+    reference = logp.float()
+    out = ops.preference_loss(ws, z, y, torch.tensor([0, n, n], device="cuda"), reference,
+                              beta=1.0, gradient=False)
+    want = (logp - reference.double()).sum().item()
+    assert abs(out.score[0].item() - want) <= n * 2.0 ** -24
