@@ -461,6 +461,7 @@ int64_t cover(int64_t n, int64_t by) { return (n + by - 1) / by; }
 int64_t power_of_two(int64_t n) { return int64_t(std::bit_ceil(uint64_t(n))); }
 
 constexpr int64_t kWorkgroups = 256;  // that fill the chip
+constexpr int64_t kFewGroups = kWorkgroups * 7 / 16;  // of the widest kernels: that take splits
 constexpr int64_t kMostSplits = 256;
 // Results of this size leave the caches to what is read twice (4 x 32768 x 512 float32 backward
 // in two launches: 362 -> 338 us); smaller ones stay, for what takes them next.
@@ -473,19 +474,20 @@ unsigned plan(Scan& a, int64_t steps, int64_t element, bool line, bool narrow) {
   if (line) {
     across = 64 / power_of_two(std::min<int64_t>(parts, 64));
   } else if (narrow) {
-    // The channels of a few sequences side by side, fewer where groups are few.  Forward of
-    // 2433 x 640 x 7 float32: 42 us by 8 lanes, 48 by 16; backward of 2000 x 1000 x 8: 77 by 8, 60
-    // by 32.
+    // The channels of a few sequences side by side, fewer where groups are few: B x 1000 x 8 float32
+    // forward and backward, B = 640: 13 and 21 us by 8 lanes, 16 and 22 by 16; 1360: 23 and 37 by
+    // 16, 26 and 40 by 32; 2000: 32 and 66 by 16, 31 and 58 by 32.
     across = a.batch_lanes < 8 ? 8 : std::min<int64_t>(4 * power_of_two(a.batch_lanes), 64);
-    while (across > 8 && cover(lanes, across) < kWorkgroups * 5 / 4) across /= 2;
+    while (across > 8 && cover(lanes, across) < kWorkgroups * 3 / 2) across /= 2;
     most_waves = 4;
   } else {
-    // 256 bytes a step; 128 where that leaves one launch enough groups and 256 would not.
-    // 8 x 4096 x 2048 bfloat16: 97 us by 128 bytes, 123 by 256 (neither read ahead);
-    // 64 x 1000 x 512 float32: 84 and 73.
+    // 256 bytes a step; 128 where its groups are at most one for every compute unit, and enough to
+    // do without splits.  B x 4096 x 128 bfloat16 forward and backward, B groups of 256 bytes, B =
+    // 48: 45 and 67 us by 256 in splits, 37 and 70 by 128; 58: 54 and 92, 39 and 84; 128: 91 and
+    // 157 by 256 without, 83 and 140 by 128; 140: 97 and 161, 113 and 170.
     across = power_of_two(std::min<int64_t>(lanes, 64));
-    if (cover(lanes, 64) < kWorkgroups * 9 / 16 && cover(lanes, 32) >= kWorkgroups * 7 / 16)
-      across = std::min<int64_t>(across, 32);
+    const int64_t halves = cover(lanes, 32);
+    if (halves >= kFewGroups && halves <= kWorkgroups) across = std::min<int64_t>(across, 32);
   }
   a.lanes = int32_t(across);
   a.groups = cover(lanes, across);
@@ -494,10 +496,15 @@ unsigned plan(Scan& a, int64_t steps, int64_t element, bool line, bool narrow) {
   const int64_t waves = std::min(power_of_two(cover(parts, depth)), most_waves);
   const int64_t block = waves * depth * steps, blocks = cover(a.time, block);
   int64_t splits = 1;
-  // Several of the narrow kernels' workgroups, with fewer registers, fit a compute unit: forward of
-  // 20 x 100000 x 7 float32 in 117 us by one, 85 by two, 83 by four.
+  // Several of the narrow and line kernels' workgroups, with fewer registers, fit a compute unit:
+  // forward of 20 x 100000 x 7 float32 in 117 us by one, 85 by two, 83 by four; of G x 5000 x 8, G
+  // groups, forward and backward, G = 160: 29 and 37 us whole, 22 and 32 in splits; 250: 30 and 39,
+  // 32 and 45; of G x 200000 x 1, G = 128: 111 and 186, 83 and 130; 150: 114 and 190, 117 and 173.
+  // A few blocks are through before a second launch begins: 100 x 1100 x 8, 5 blocks, 10 and 13 us
+  // whole, 12 and 15 in splits; 100 x 2100 x 8, 9 blocks, 15 and 19, 13 and 15.
+  const int64_t few = narrow ? kWorkgroups * 3 / 4 : line ? kWorkgroups * 9 / 16 : kFewGroups;
   const int64_t wanted = line || narrow ? 4 * kWorkgroups : kWorkgroups;
-  if (a.groups < kWorkgroups * 7 / 16)
+  if (a.groups < few && blocks >= 6)
     splits = std::min({cover(wanted, a.groups), blocks, kMostSplits});
   a.split_steps = cover(blocks, splits) * block;
   a.splits = int32_t(cover(a.time, a.split_steps));
