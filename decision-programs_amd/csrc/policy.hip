@@ -11,12 +11,11 @@
 // A class whose margin is -infinity has probability zero and adds nothing; a row
 // without any other class is not counted.
 //
-// Held in 64 bits: sums of exponentials, log p_y, its differences to old and reference
-// log-probabilities (the difference of two of about -10 that differ by 0.1 keeps 5 digits in
-// 32), e^d - 1 - d and the sums over sequences.  In 32 bits, since each is a rounding beside those
-// of the outputs: an element's exponential, of which a sum has the mean error; the logarithm
-// of a sum; sum e^d d, and the entropy with it; the ratio; what a loss and its slopes are
-// put together from.
+// Held in 64 bits: sums of exponentials and their logarithms, log p_y, its differences to old
+// and reference log-probabilities (the difference of two of about -10 that differ by 0.1 keeps 5
+// digits in 32), e^d - 1 - d and the sums over sequences.  In 32 bits, since each is a rounding
+// beside those of the outputs: an element's exponential, of which a sum has the mean error; sum
+// e^d d, and the entropy with it; the ratio; what a loss and its slopes are put together from.
 //
 // Bound by HBM where there is work for the whole chip (16-bit rows of up to 512 vectors: by
 // vector instructions), so each row is read once if it can be held: in LDS and a thread's
@@ -40,13 +39,26 @@ constexpr double kLog2eLoss = 1.0 - double(kLog2e) * kLn2d;
 // Below this power of two everything is 0.
 constexpr float kNoPower = -200.0f;
 
-// log s, to about 2^-23 of itself: s is at least 1 but for roundings, so that a sum near 1, of
-// a row that one class has almost all of, goes by what is beside that 1.
+// log s, to 2^-39 of itself: s = 2^e m with m about 1, log m = 2 atanh((m - 1) / (m + 1)), whose
+// first term left out is ((m - 1) / (m + 1))^14 / 15 < 2^-39.  s is at least 1 but for roundings: a
+// sum near 1, of a row that one class has almost all of, goes by what is beside that 1.
 __device__ __forceinline__ double log_sum(double s) {
-  if (s < 2.0) return double(log1pf(float(s - 1.0)));
   int e;
-  const double f = frexp(s, &e);
-  return double(e) * kLn2d + double(logf(float(f)));
+  double m = frexp(s, &e);
+  const bool low = m < 0.70710678118654752;
+  m = low ? 2.0 * m : m;
+  e = low ? e - 1 : e;
+  const double rest = m - 1.0, d = 2.0 + rest;
+  double r = __builtin_amdgcn_rcp(d);
+  r = fma(fma(-d, r, 1.0), r, r);
+  const double t = rest * r, q = t * t;
+  double p = 1.0 / 13.0;
+  p = fma(p, q, 1.0 / 11.0);
+  p = fma(p, q, 1.0 / 9.0);
+  p = fma(p, q, 1.0 / 7.0);
+  p = fma(p, q, 1.0 / 5.0);
+  p = fma(p, q, 1.0 / 3.0);
+  return fma(double(e), kLn2d, 2.0 * fma(t * q, p, t));
 }
 
 // e^x with what x loses in 32 bits put right.

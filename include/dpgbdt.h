@@ -380,8 +380,8 @@ int dp_update_margin(dp_workspace ws, const uint32_t* ridx, const int64_t* begin
  * hessian are 0.  A class whose margin is -infinity has probability 0 and
  * gradient 0; a row with no other class is not counted either.  NaN in a counted
  * row reaches that row's outputs only (and its pair's).  Sums of exponentials,
- * log p_y and its differences are held in 64 bits (sums of 16-bit margins in 32
- * over 8 classes); exponentials, the logarithm of a sum and what a loss is put
+ * their logarithms, log p_y and its differences are held in 64 bits (sums of
+ * 16-bit margins in 32 over 8 classes); exponentials and what a loss is put
  * together from are rounded to 32 bits.  The same call gives the same bits every
  * time.  log p_y and H of a row of at most 8192 whole vectors of 16 bytes are the
  * same bits in every call.  Longer rows are added up in pieces that go by the

@@ -506,6 +506,23 @@ def test_gradients_by_the_roundings_they_have(ws, device, k):
                 + np.abs(c) * taken * 2.0 ** -24, "grad")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("k", [2, 3, 5, 7, 10, 31, 33, 100, 1000, 1500, 3000, 9001, 33001, 70001])
+def test_the_logarithm_of_a_sum(ws, device, k, dtype):
+    """Equal margins: the sum is k without an error, and a sequence of one row scores -log k less
+    a reference of nearly that, of which 2^-39 of the logarithm is left."""
+    import torch
+    from dpgbdt import ops
+
+    z = torch.full((1, k), 1.5, dtype=getattr(torch, dtype), device="cuda")
+    y = torch.zeros(1, dtype=torch.int64, device="cuda")
+    reference = torch.tensor([-np.log(k)], dtype=torch.float32, device="cuda")
+    out = ops.preference_loss(ws, z, y, torch.tensor([0, 1, 1], device="cuda"), reference,
+                              beta=1.0, gradient=False)
+    want = -np.log(float(k)) - reference.double().item()
+    assert abs(out.score[0].item() - want) <= 2.0 ** -39 * np.log(k) + 2.0 ** -24 * abs(want)
+
+
 def test_log_probabilities_of_a_sequence_have_no_common_error(ws, device):
     """What all rows are off by in the same way adds up over a sequence.  log2(e) loses 1.3e-8 of
     itself in 32 bits; by 0.8 of probability at e^-10.4 it would be 1.1e-7 a row, against the 2^-25
