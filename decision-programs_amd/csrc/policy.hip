@@ -660,7 +660,7 @@ __global__ __launch_bounds__(kThreads) void short_row_kernel(Rows a, uint32_t ma
 // The last vector of a row is one of the lanes' last kLast ones: there are more than
 // (NV - kLast) LANES and at most NV LANES.  It ends with the row, so that it holds elements of the
 // one before again.
-// Scoring 1.9 million x 64 float32: 91 us, 5.6 TB/s (one batch a wave: 206); 80,000 x 1500: 79 us
+// Scoring 1.9 million x 64 float32: 90 us, 5.6 TB/s (one batch a wave: 206); 80,000 x 1500: 79 us
 // (a workgroup a row: 125).  16-bit rows are bound by vector instructions, at 3 to 4.5 TB/s.
 template <int LANES, int NV>
 constexpr int kBatches = NV == 1 ? (LANES < 16 ? LANES : 16) : NV == 2 ? 8 : NV > 4 ? 1 : 12 / NV;
@@ -804,7 +804,7 @@ struct Span {
 // ---------------------------------------------------------------------------
 // The row is read once, as NV vectors a thread and the single elements beside them, one a thread;
 // statistics and gradient come from the registers.  8192 x 32768 bfloat16 policy loss: 209 us, 5.1
-// TB/s, the vector units 70 % busy; scoring 4096 x 50021 85 us, 84 % busy.  Workgroups of 256 to
+// TB/s, the vector units 72 % busy; scoring 4096 x 50021 85 us, 82 % busy.  Workgroups of 256 to
 // 512 threads with many registers, of which 2 to 4 on a compute unit are in different phases, beat
 // one of 1024 (225 us).
 // Waves a SIMD: as many as leave registers for the vectors and the row's 64-bit numbers.
